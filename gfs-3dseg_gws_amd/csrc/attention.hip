@@ -570,3 +570,7 @@ extern "C" int gfs3d_attention_dropout_mask(int B, int N, float p_drop, unsigned
     GFS3D_LAUNCH_CHECK("attn_mask_kernel");
     return GFS3D_OK;
 }
+
+// the operators of a layer over serialised points: window attention (K7), rotary positions (K8), RMS norm (K9)
+#include "window_attention.h"
+#include "row_ops.h"

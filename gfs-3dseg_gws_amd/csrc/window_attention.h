@@ -1,0 +1,945 @@
+// K7: attention with a sliding window and a few first tokens that stay visible (sinks), over serialised points
+//
+//     o_i = sum_j p_ij v_j,   p_i. = softmax over the visible j of  scale q_i . k_j
+//     j visible to i:  i, j < length  and  j <= i + right  and  (j >= i - left  or  j < sinks)
+//
+// q (B, N, H, D), k / v (B, N, G, D) point-major with any strides, head h reads key head h / (H / G); fp32, bf16 or half.
+// Part of attention.hip (the operand images and the transposed LDS read are those of K5 there).
+//
+// Forward: a wave owns one unit = 32 queries of one head (the QUERY on the lane, S^T = K Q^T, so that a query's running maximum,
+// sum and accumulators are in-lane), the four waves of a workgroup own consecutive units with the heads of one key head innermost:
+// they share every staged key tile.  Tiles outside all four windows are never staged, tiles outside a wave's own window cost it
+// nothing but the barrier, and only tiles that a window edge, the diagonal or the length cuts pay for the element mask.
+// Backward: dQ with the query on the lane (it also leaves delta_i = dout_i . o_i), dK / dV with the key on the lane, looping over the
+// heads of the key head; what the sinks receive from queries beyond their window (all rows of a long sequence) is summed by
+// its own kernel in row chunks, and the chunks are joined, in order, where dK / dV of those keys are written.  No atomics.
+// Scores, softmax statistics, accumulators and all sums over heads or chunks are fp32.  Probabilities and dS are rounded to the operand
+// type of the matrix cores: bf16 / half for those tensors, exact 3-way bf16 splits (PREC_X6) for fp32; the gradients of half
+// tensors take two bf16 pieces (PREC_X3), whose range is fp32's - a mean loss underflows in half.
+
+namespace gfs3d {
+namespace {
+
+struct WaStride { long long b, r, h; };          // elements between sequences, rows, heads
+struct WaArgs {
+    const void *q, *k, *v, *out, *dout;
+    WaStride qs, ks, vs, gs;                      // gs: dout
+    const int *lengths;                           // (B) device, or NULL: all S
+    float *lse, *delta;                           // (B, H, N): log2-sum-exp2 of the scaled scores; dout . out
+    float *part;                                  // partial sums (sinks' gradients / split keys)
+    int B, N, S, H, G, HG, D;                     // N query rows, S keys per sequence
+    int left, right, sinks;
+    int nblk;                                     // workgroups per (sequence, key head)
+    int nst, nchunk;                              // sinks' key tiles, row chunks of their gradient
+    float scale, c;                               // c = scale log2(e)
+};
+
+template <class T> struct WaT;
+template <> struct WaT<float> { static constexpr int PF = PREC_X6, PB = PREC_X6, KT = 32; };
+template <> struct WaT<__bf16> { static constexpr int PF = PREC_BF16, PB = PREC_BF16, KT = 64; };
+template <> struct WaT<_Float16> { static constexpr int PF = PREC_F16, PB = PREC_X3, KT = 64; };
+
+// eight consecutive channels as they lie in memory
+template <class T> struct WaRaw { uint4 a; };
+template <> struct WaRaw<float> { float4 a, b; };
+template <class T> __device__ __forceinline__ WaRaw<T> wa_zero() { return WaRaw<T>{make_uint4(0u, 0u, 0u, 0u)}; }
+template <> __device__ __forceinline__ WaRaw<float> wa_zero<float>() { return WaRaw<float>{make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)}; }
+template <class T> __device__ __forceinline__ WaRaw<T> wa_load8(const T *p) { return *reinterpret_cast<const WaRaw<T> *>(p); }
+template <class T> __device__ __forceinline__ void wa_floats(const WaRaw<T> &r, float (&v)[8])
+{
+    if constexpr (sizeof(T) == 4) {
+        v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w; v[4] = r.b.x; v[5] = r.b.y; v[6] = r.b.z; v[7] = r.b.w;
+    } else {
+        typedef T Tx8 __attribute__((ext_vector_type(8)));
+        const Tx8 x = __builtin_bit_cast(Tx8, r.a);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (float)x[e];
+    }
+}
+template <class T, int PREC> __device__ __forceinline__ void wa_pieces(const WaRaw<T> &r, uint4 (&f)[Mx<PREC>::NP])
+{
+    if constexpr (sizeof(T) == 2 && Mx<PREC>::NP == 1) {
+        f[0] = r.a;
+    } else {
+        float v[8];
+        wa_floats<T>(r, v);
+        mm_pieces8<PREC>(v, f);
+    }
+}
+template <class T> __device__ __forceinline__ void wa_store4(T *p, float a, float b, float c, float d)
+{
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4 *>(p) = make_float4(a, b, c, d);
+    else {
+        constexpr int P = WaT<T>::PF;
+        *reinterpret_cast<uint2 *>(p) = make_uint2(mm_pack2<P>(a, b), mm_pack2<P>(c, d));
+    }
+}
+
+// images: [plane][row][2 DP bytes | 16 pad]: the pad turns 16 consecutive rows of one 16-byte column onto 64 different banks
+template <int DP> struct WaImg {
+    static constexpr int ROWB = 2 * DP + 16;
+    template <int R> static constexpr int plane() { return R * ROWB; }
+};
+template <int PREC, int DP, int R>
+__device__ __forceinline__ void wa_rowfrag(const unsigned char *img, int j, int h, int kb, uint4 (&f)[Mx<PREC>::NP])
+{
+#pragma unroll
+    for (int p = 0; p < Mx<PREC>::NP; ++p)
+        f[p] = *reinterpret_cast<const uint4 *>(img + p * WaImg<DP>::template plane<R>() + j * WaImg<DP>::ROWB + 32 * kb + 16 * h);
+}
+// rows = channels 32 dt + (lane & 31), k-step s: positions at_drow(8 s + e, h) of the 32 rows at `img` (see at_trfrag)
+template <int PREC, int DP, int R>
+__device__ __forceinline__ void wa_trfrag(const unsigned char *img, int lane, int dt, int s, uint4 (&f)[Mx<PREC>::NP])
+{
+    constexpr int ROWB = WaImg<DP>::ROWB;
+    const int h = lane >> 5, g1 = (lane >> 4) & 1, q = (lane >> 2) & 3, p4 = lane & 3;
+    const unsigned char *base = img + (16 * s + 4 * h + q) * ROWB + 2 * (32 * dt + 16 * g1 + 4 * p4);
+#pragma unroll
+    for (int p = 0; p < Mx<PREC>::NP; ++p) {
+        const unsigned char *bp = base + p * WaImg<DP>::template plane<R>();
+        const at_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)(bp));
+        const at_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((at_lds_s16x4 *)(bp + 8 * ROWB));
+        const uint2 a = __builtin_bit_cast(uint2, lo), b = __builtin_bit_cast(uint2, hi);
+        f[p] = make_uint4(a.x, a.y, b.x, b.y);
+    }
+}
+// the per-wave constant operand: lane (column, half h) holds channels 16 kb + 8 h .. of its row (zeros past D or where !ok)
+template <class T, int PREC, int DP>
+__device__ __forceinline__ void wa_colfrags(const T *row, bool ok, int D, int h, uint4 (&f)[DP / 16][Mx<PREC>::NP])
+{
+#pragma unroll
+    for (int kb = 0; kb < DP / 16; ++kb) {
+        const int ch = 16 * kb + 8 * h;
+        WaRaw<T> r = wa_zero<T>();
+        if (ok && ch < D) r = wa_load8<T>(row + ch);
+        wa_pieces<T, PREC>(r, f[kb]);
+    }
+}
+
+// R rows of a (rows, D) matrix staged by NT threads: thread t takes the 8-channel chunks t, t + NT, ..
+template <class T, int DP, int R, int NT> struct WaStage {
+    static constexpr int CPR = DP / 8, NCH = (R * CPR + NT - 1) / NT;
+    static constexpr bool RAGGED = R * CPR % NT != 0;
+    WaRaw<T> r[NCH];
+    // rows [row0, row0 + R) at `base` (row row0), rows >= end and channels >= D read as zeros
+    __device__ __forceinline__ void load(const T *base, long long stride, int row0, int end, int D, int t)
+    {
+#pragma unroll
+        for (int n = 0; n < NCH; ++n) {
+            const int c = t + n * NT, row = c / CPR, ch = 8 * (c % CPR);
+            r[n] = wa_zero<T>();
+            if ((!RAGGED || c < R * CPR) && row0 + row < end && ch < D) r[n] = wa_load8<T>(base + (long long)row * stride + ch);
+        }
+    }
+    template <int PREC> __device__ __forceinline__ void put(unsigned char *img, int t) const
+    {
+#pragma unroll
+        for (int n = 0; n < NCH; ++n) {
+            const int c = t + n * NT, row = c / CPR, ch = c % CPR;
+            uint4 f[Mx<PREC>::NP];
+            wa_pieces<T, PREC>(r[n], f);
+            if (!RAGGED || c < R * CPR) {
+#pragma unroll
+                for (int p = 0; p < Mx<PREC>::NP; ++p)
+                    *reinterpret_cast<uint4 *>(img + p * WaImg<DP>::template plane<R>() + row * WaImg<DP>::ROWB + 16 * ch) = f[p];
+            }
+        }
+    }
+};
+
+// (x of the lower half, x of the upper half) in every lane: one register's upper half changes places with another's lower half
+__device__ __forceinline__ float2 wa_halves(float x)
+{
+    const unsigned a = __builtin_bit_cast(unsigned, x);
+    const auto r = __builtin_amdgcn_permlane32_swap(a, a, false, false);
+    const unsigned lo = r[0], hi = r[1];              // (a bit cast of r[1] itself reads r[0])
+    return make_float2(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
+__device__ __forceinline__ float wa_max32(float x) { const float2 r = wa_halves(x); return fmaxf(r.x, r.y); }
+__device__ __forceinline__ float wa_sum32(float x) { const float2 r = wa_halves(x); return r.x + r.y; }
+__device__ __forceinline__ int wa_length(const int *lengths, int b, int S) { return lengths ? min(max(lengths[b], 0), S) : S; }
+// workgroups go to the 8 XCDs in turn: give each XCD (its own L2) a contiguous run, so that neighbours share their key tiles there
+__device__ __forceinline__ unsigned wa_order(unsigned id, unsigned total)
+{
+    const unsigned per = total / 8, x = id & 7;
+    return id < per * 8 ? x * per + id / 8 : id;
+}
+constexpr float WA_LAZY = 8.f;        // the running maximum may lag the true one by 2^8: p, its sum and its products stay in range in fp32 and half
+
+// ------------------------------------------------------------------ forward
+template <class T, int DP>
+__global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_fwd_kernel(const WaArgs g, T *__restrict__ out)
+{
+    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, KT = WaT<T>::KT, SUB = KT / 32, IMG = NP * KT * WaImg<DP>::ROWB;
+    constexpr int ROWB = WaImg<DP>::ROWB, ND = DP / 32;
+    extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
+    unsigned char *Kimg = at_smem, *Vimg = at_smem + 2 * IMG;
+    const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    const unsigned bid = wa_order(blockIdx.x, gridDim.x);
+    const int blk = bid % g.nblk, bg = bid / g.nblk, b = bg / g.G, gi = bg % g.G;
+    const int len = wa_length(g.lengths, b, g.N), nqt = (g.N + 31) / 32;
+    const int u = blk * 4 + wv, qt = u / g.HG, head = gi * g.HG + u % g.HG, q0 = qt * 32, qi = q0 + j;
+    const bool live = q0 < len;                         // this wave has rows (qt < nqt follows)
+    const int qa = blk * 4 / g.HG * 32, qb = min((blk * 4 + 3) / g.HG, nqt - 1) * 32 + 31;       // the workgroup's rows
+    const T *kb_ = (const T *)g.k + b * g.ks.b + gi * g.ks.h, *vb = (const T *)g.v + b * g.vs.b + gi * g.vs.h;
+
+    uint4 qp[DP / 16][NP];
+    wa_colfrags<T, PREC, DP>((const T *)g.q + b * g.qs.b + (long long)qi * g.qs.r + head * g.qs.h, qi < len, g.D, h, qp);
+    float m = -__builtin_inff(), mc = 0.f, l = 0.f;      // running maximum (raw scores), c m (0 while there is none), this half's sum
+    f32x16 O[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[d][r] = 0.f;
+
+    const int tlo = max(0, qa - g.left) / KT, thi = min(len - 1, qb + g.right) / KT;
+    const int nsink = min((min(g.sinks, len) + KT - 1) / KT, tlo);
+    const int nt = qa < len ? nsink + thi - tlo + 1 : 0;
+    const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right);
+    const float thr = WA_LAZY / g.c;
+    WaStage<T, DP, KT, 256> sk, sv;
+    auto row0 = [&](int tt) { return (tt < nsink ? tt : tlo + tt - nsink) * KT; };
+    auto load = [&](int tt) {
+        const int r0 = row0(tt);
+        sk.load(kb_ + (long long)r0 * g.ks.r, g.ks.r, r0, len, g.D, t);
+        sv.load(vb + (long long)r0 * g.vs.r, g.vs.r, r0, len, g.D, t);
+    };
+    if (nt > 0) {
+        load(0);
+        sk.template put<PREC>(Kimg, t);
+        sv.template put<PREC>(Vimg, t);
+    }
+    __syncthreads();
+    for (int tt = 0; tt < nt; ++tt) {
+        const int cur = tt & 1, j0 = row0(tt);
+        const unsigned char *Kc = Kimg + cur * IMG, *Vc = Vimg + cur * IMG;
+        if (tt + 1 < nt) load(tt + 1);
+        if (live && j0 <= whi && (j0 + KT > wlo || j0 < g.sinks)) {
+            f32x16 acc[SUB];
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[s][r] = 0.f;
+#pragma unroll
+                for (int kb = 0; kb < DP / 16; ++kb) {
+                    uint4 ak[NP];
+                    wa_rowfrag<PREC, DP, KT>(Kc, 32 * s + j, h, kb, ak);
+                    mm_mac<PREC>(ak, qp[kb], acc[s]);
+                }
+            }
+            if (!(j0 + KT <= len && j0 + KT - 1 <= q0 + g.right && (j0 >= q0 + 31 - g.left || j0 + KT <= g.sinks))) {
+#pragma unroll
+                for (int s = 0; s < SUB; ++s)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int jj = j0 + 32 * s + at_drow(r, h);
+                        const bool ok = jj < len && jj <= qi + g.right && (jj >= qi - g.left || jj < g.sinks);
+                        acc[s][r] = ok ? acc[s][r] : -__builtin_inff();
+                    }
+            }
+            float tmax = acc[0][0];
+#pragma unroll
+            for (int s = 0; s < SUB; ++s)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, acc[s][r]);
+            tmax = wa_max32(tmax);
+            if (__ballot(tmax > m + thr) != 0ull) {
+                const float m_new = fmaxf(m, tmax), mc_new = m_new == -__builtin_inff() ? 0.f : m_new * g.c;
+                const float sc = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mc - mc_new);
+                m = m_new;
+                mc = mc_new;
+                l *= sc;
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) O[d][r] *= sc;
+            }
+#pragma unroll
+            for (int s = 0; s < SUB; ++s) {
+                float pd[16];
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    pd[r] = __builtin_amdgcn_exp2f(fmaf(acc[s][r], g.c, -mc));
+                    l += pd[r];
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    uint4 pp[NP], av[NP];
+                    at_regfrag<PREC>(pd, ks, pp);
+#pragma unroll
+                    for (int d = 0; d < ND; ++d) {
+                        wa_trfrag<PREC, DP, KT>(Vc + 32 * s * ROWB, lane, d, ks, av);
+                        mm_mac<PREC>(av, pp, O[d]);
+                    }
+                }
+            }
+        }
+        if (tt + 1 < nt) { sk.template put<PREC>(Kimg + (cur ^ 1) * IMG, t); sv.template put<PREC>(Vimg + (cur ^ 1) * IMG, t); }
+        __syncthreads();
+    }
+    if (qi < g.N && qt < nqt) {
+        const float lt = wa_sum32(l), inv = lt > 0.f && qi < len ? 1.f / lt : (lt != lt ? lt : 0.f);
+        T *ob = out + (((size_t)b * g.N + qi) * g.H + head) * g.D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int ch = 32 * d + at_drow(r, h);
+                if (ch < g.D) wa_store4<T>(ob + ch, O[d][r] * inv, O[d][r + 1] * inv, O[d][r + 2] * inv, O[d][r + 3] * inv);
+            }
+        if (g.lse && h == 0) g.lse[((size_t)b * g.H + head) * g.N + qi] = lt > 0.f && qi < len ? mc + __builtin_amdgcn_logf(lt) : __builtin_inff();
+    }
+}
+
+// ------------------------------------------------------------------ backward, query side: dQ and delta
+template <class T, int DP>
+__global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_bwd_dq_kernel(const WaArgs g, T *__restrict__ dq)
+{
+    constexpr int PREC = WaT<T>::PB, NP = Mx<PREC>::NP, KT = 32, IMG = NP * KT * WaImg<DP>::ROWB, ND = DP / 32;
+    extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
+    unsigned char *Kimg = at_smem, *Vimg = at_smem + 2 * IMG;
+    const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    const unsigned bid = wa_order(blockIdx.x, gridDim.x);
+    const int blk = bid % g.nblk, bg = bid / g.nblk, b = bg / g.G, gi = bg % g.G;
+    const int len = wa_length(g.lengths, b, g.N), nqt = (g.N + 31) / 32;
+    const int u = blk * 4 + wv, qt = u / g.HG, head = gi * g.HG + u % g.HG, q0 = qt * 32, qi = q0 + j;
+    const bool live = q0 < len, mine = qi < len;
+    const int qa = blk * 4 / g.HG * 32, qb = min((blk * 4 + 3) / g.HG, nqt - 1) * 32 + 31;
+    const T *kb_ = (const T *)g.k + b * g.ks.b + gi * g.ks.h, *vb = (const T *)g.v + b * g.vs.b + gi * g.vs.h;
+
+    uint4 qp[DP / 16][NP], gp[DP / 16][NP];
+    wa_colfrags<T, PREC, DP>((const T *)g.q + b * g.qs.b + (long long)qi * g.qs.r + head * g.qs.h, mine, g.D, h, qp);
+    float dl = 0.f;
+    {
+        const T *grow = (const T *)g.dout + b * g.gs.b + (long long)qi * g.gs.r + head * g.gs.h;
+        const T *orow = (const T *)g.out + (((size_t)b * g.N + qi) * g.H + head) * g.D;
+#pragma unroll
+        for (int kb = 0; kb < DP / 16; ++kb) {
+            const int ch = 16 * kb + 8 * h;
+            WaRaw<T> rg = wa_zero<T>(), ro = wa_zero<T>();
+            if (mine && ch < g.D) { rg = wa_load8<T>(grow + ch); ro = wa_load8<T>(orow + ch); }
+            float fg[8], fo[8];
+            wa_floats<T>(rg, fg);
+            wa_floats<T>(ro, fo);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dl = fmaf(fg[e], fo[e], dl);
+            wa_pieces<T, PREC>(rg, gp[kb]);
+        }
+        dl = wa_sum32(dl);
+    }
+    const size_t row = ((size_t)b * g.H + head) * g.N + qi;
+    const float Lq = mine ? g.lse[row] : __builtin_inff();
+    if (qi < g.N && qt < nqt && h == 0) g.delta[row] = dl;
+    f32x16 A[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) A[d][r] = 0.f;
+
+    const int tlo = max(0, qa - g.left) / KT, thi = min(len - 1, qb + g.right) / KT;
+    const int nsink = min((min(g.sinks, len) + KT - 1) / KT, tlo);
+    const int nt = qa < len ? nsink + thi - tlo + 1 : 0;
+    const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right);
+    WaStage<T, DP, KT, 256> sk, sv;
+    auto row0 = [&](int tt) { return (tt < nsink ? tt : tlo + tt - nsink) * KT; };
+    auto load = [&](int tt) {
+        const int r0 = row0(tt);
+        sk.load(kb_ + (long long)r0 * g.ks.r, g.ks.r, r0, len, g.D, t);
+        sv.load(vb + (long long)r0 * g.vs.r, g.vs.r, r0, len, g.D, t);
+    };
+    if (nt > 0) {
+        load(0);
+        sk.template put<PREC>(Kimg, t);
+        sv.template put<PREC>(Vimg, t);
+    }
+    __syncthreads();
+    for (int tt = 0; tt < nt; ++tt) {
+        const int cur = tt & 1, j0 = row0(tt);
+        const unsigned char *Kc = Kimg + cur * IMG, *Vc = Vimg + cur * IMG;
+        if (tt + 1 < nt) load(tt + 1);
+        if (live && j0 <= whi && (j0 + KT > wlo || j0 < g.sinks)) {
+            f32x16 acc, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { acc[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+            for (int kb = 0; kb < DP / 16; ++kb) {
+                uint4 ak[NP], av[NP];
+                wa_rowfrag<PREC, DP, KT>(Kc, j, h, kb, ak);
+                wa_rowfrag<PREC, DP, KT>(Vc, j, h, kb, av);
+                mm_mac<PREC>(ak, qp[kb], acc);
+                mm_mac<PREC>(av, gp[kb], dp);
+            }
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(acc[r], g.c, -Lq)) * (dp[r] - dl);
+            if (!(j0 + KT <= len && q0 + 32 <= len && j0 + KT - 1 <= q0 + g.right && (j0 >= q0 + 31 - g.left || j0 + KT <= g.sinks))) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int jj = j0 + at_drow(r, h);
+                    const bool ok = mine && jj < len && jj <= qi + g.right && (jj >= qi - g.left || jj < g.sinks);
+                    ds[r] = ok ? ds[r] : 0.f;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                uint4 dsp[NP], ak[NP];
+                at_regfrag<PREC>(ds, s, dsp);
+#pragma unroll
+                for (int d = 0; d < ND; ++d) {
+                    wa_trfrag<PREC, DP, KT>(Kc, lane, d, s, ak);
+                    mm_mac<PREC>(ak, dsp, A[d]);
+                }
+            }
+        }
+        if (tt + 1 < nt) { sk.template put<PREC>(Kimg + (cur ^ 1) * IMG, t); sv.template put<PREC>(Vimg + (cur ^ 1) * IMG, t); }
+        __syncthreads();
+    }
+    if (qi < g.N && qt < nqt) {
+        T *ob = dq + (((size_t)b * g.N + qi) * g.H + head) * g.D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int ch = 32 * d + at_drow(r, h);
+                if (ch < g.D) wa_store4<T>(ob + ch, A[d][r] * g.scale, A[d][r + 1] * g.scale, A[d][r + 2] * g.scale, A[d][r + 3] * g.scale);
+            }
+    }
+}
+
+// one 32-query tile against the wave's 32 keys: K += dS^T q, V += P^T dout (unscaled).  SINK: pairs beyond the window (j < sinks,
+// j < i - left), otherwise the window's
+template <class T, int PREC, int DP, bool SINK>
+__device__ __forceinline__ void wa_dkv_tile(const WaArgs &g, const unsigned char *Qc, const unsigned char *Gc, const float *Ls, const float *Ds,
+                                            int p0, int k0, int len, int lane, const uint4 (&kp)[DP / 16][Mx<PREC>::NP],
+                                            const uint4 (&vp)[DP / 16][Mx<PREC>::NP], f32x16 (&AK)[DP / 32], f32x16 (&AV)[DP / 32])
+{
+    constexpr int NP = Mx<PREC>::NP, ND = DP / 32;
+    const int j = lane & 31, h = lane >> 5, ki = k0 + j;
+    f32x16 acc, dp;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) { acc[r] = 0.f; dp[r] = 0.f; }
+#pragma unroll
+    for (int kb = 0; kb < DP / 16; ++kb) {
+        uint4 aq[NP], ag[NP];
+        wa_rowfrag<PREC, DP, 32>(Qc, j, h, kb, aq);
+        wa_rowfrag<PREC, DP, 32>(Gc, j, h, kb, ag);
+        mm_mac<PREC>(aq, kp[kb], acc);
+        mm_mac<PREC>(ag, vp[kb], dp);
+    }
+    float pd[16], ds[16];
+#pragma unroll
+    for (int r4 = 0; r4 < 16; r4 += 4) {
+        const float4 L4 = *reinterpret_cast<const float4 *>(Ls + at_drow(r4, h)), D4 = *reinterpret_cast<const float4 *>(Ds + at_drow(r4, h));
+        const float lv[4] = {L4.x, L4.y, L4.z, L4.w}, dv[4] = {D4.x, D4.y, D4.z, D4.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            pd[r4 + e] = __builtin_amdgcn_exp2f(fmaf(acc[r4 + e], g.c, -lv[e]));
+            ds[r4 + e] = pd[r4 + e] * (dp[r4 + e] - dv[e]);
+        }
+    }
+    const bool whole = SINK ? p0 + 32 <= len && k0 + 32 <= min(g.sinks, len) && k0 + 31 < p0 - g.left
+                            : p0 + 32 <= len && k0 + 32 <= len && k0 + 31 <= p0 + g.right && k0 >= p0 + 31 - g.left;
+    if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int i = p0 + at_drow(r, h);
+            const bool ok = i < len && ki < len && (SINK ? ki < g.sinks && ki < i - g.left : ki <= i + g.right && ki >= i - g.left);
+            pd[r] = ok ? pd[r] : 0.f;
+            ds[r] = ok ? ds[r] : 0.f;
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        uint4 bp[NP], bs[NP], af[NP];
+        at_regfrag<PREC>(pd, s, bp);
+        at_regfrag<PREC>(ds, s, bs);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) {
+            wa_trfrag<PREC, DP, 32>(Gc, lane, d, s, af);
+            mm_mac<PREC>(af, bp, AV[d]);
+            wa_trfrag<PREC, DP, 32>(Qc, lane, d, s, af);
+            mm_mac<PREC>(af, bs, AK[d]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ backward, key side: dK, dV
+template <class T, int DP>
+__global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(const WaArgs g, T *__restrict__ dk, T *__restrict__ dv)
+{
+    constexpr int PREC = WaT<T>::PB, NP = Mx<PREC>::NP, IMG = NP * 32 * WaImg<DP>::ROWB, ND = DP / 32;
+    extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
+    unsigned char *Qimg = at_smem, *Gimg = at_smem + 2 * IMG;
+    float (*Ls)[32] = reinterpret_cast<float (*)[32]>(at_smem + 4 * IMG), (*Ds)[32] = Ls + 2;       // [2][32] each
+    const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    const unsigned bid = wa_order(blockIdx.x, gridDim.x);
+    const int blk = bid % g.nblk, bg = bid / g.nblk, b = bg / g.G, gi = bg % g.G;
+    const int len = wa_length(g.lengths, b, g.N), kt = blk * 4 + wv, k0 = kt * 32, ki = k0 + j;
+    const int ka = blk * 128, kz = min(ka + 127, len - 1);
+
+    uint4 kp[DP / 16][NP], vp[DP / 16][NP];
+    wa_colfrags<T, PREC, DP>((const T *)g.k + b * g.ks.b + (long long)ki * g.ks.r + gi * g.ks.h, ki < len, g.D, h, kp);
+    wa_colfrags<T, PREC, DP>((const T *)g.v + b * g.vs.b + (long long)ki * g.vs.r + gi * g.vs.h, ki < len, g.D, h, vp);
+    f32x16 AK[ND], AV[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { AK[d][r] = 0.f; AV[d][r] = 0.f; }
+
+    const int tlo = max(0, ka - g.right) / 32, thi = min(len - 1, kz + g.left) / 32, per = thi - tlo + 1;
+    const int nt = ka < len ? per * g.HG : 0;
+    WaStage<T, DP, 32, 256> sq, sg;
+    float l1 = 0.f;
+    auto load = [&](int tt) {
+        const int head = gi * g.HG + tt / per, r0 = (tlo + tt % per) * 32;
+        sq.load((const T *)g.q + b * g.qs.b + (long long)r0 * g.qs.r + head * g.qs.h, g.qs.r, r0, len, g.D, t);
+        sg.load((const T *)g.dout + b * g.gs.b + (long long)r0 * g.gs.r + head * g.gs.h, g.gs.r, r0, len, g.D, t);
+        if (t < 64) l1 = r0 + (t & 31) < len ? (t < 32 ? g.lse : g.delta)[((size_t)b * g.H + head) * g.N + r0 + (t & 31)] : 0.f;
+    };
+    auto put = [&](int buf) {
+        sq.template put<PREC>(Qimg + buf * IMG, t);
+        sg.template put<PREC>(Gimg + buf * IMG, t);
+        if (t < 64) (t < 32 ? Ls : Ds)[buf][t & 31] = l1;
+    };
+    if (nt > 0) { load(0); put(0); }
+    __syncthreads();
+    for (int tt = 0; tt < nt; ++tt) {
+        const int cur = tt & 1, p0 = (tlo + tt % per) * 32;
+        if (tt + 1 < nt) load(tt + 1);
+        if (k0 < len && p0 + 31 >= k0 - g.right && p0 <= k0 + 31 + g.left)
+            wa_dkv_tile<T, PREC, DP, false>(g, Qimg + cur * IMG, Gimg + cur * IMG, Ls[cur], Ds[cur], p0, k0, len, lane, kp, vp, AK, AV);
+        if (tt + 1 < nt) put(cur ^ 1);
+        __syncthreads();
+    }
+    if (kt < g.nst) {                                     // the sinks' share from rows beyond their window, chunk by chunk
+        const float *pt = g.part + ((size_t)bg * g.nst + kt) * g.nchunk * (2 * DP * 32) + j;
+        for (int ch = 0; ch < g.nchunk; ++ch, pt += 2 * DP * 32)
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    AK[d][r] += pt[(32 * d + at_drow(r, h)) * 32];
+                    AV[d][r] += pt[(DP + 32 * d + at_drow(r, h)) * 32];
+                }
+    }
+    if (ki < g.N) {
+        const size_t o = (((size_t)b * g.N + ki) * g.G + gi) * g.D;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const int ch = 32 * d + at_drow(r, h);
+                if (ch >= g.D) continue;
+                wa_store4<T>(dk + o + ch, AK[d][r] * g.scale, AK[d][r + 1] * g.scale, AK[d][r + 2] * g.scale, AK[d][r + 3] * g.scale);
+                wa_store4<T>(dv + o + ch, AV[d][r], AV[d][r + 1], AV[d][r + 2], AV[d][r + 3]);
+            }
+    }
+}
+
+// what 32 sink keys receive from the rows of one chunk that lie beyond their window: part[bg][tile][chunk][dK | dV][channel][key]
+template <class T, int DP> constexpr int WA_SINK_NW = DP == 128 && Mx<WaT<T>::PB>::NP == 3 ? 2 : 4;       // waves: what LDS holds
+template <class T, int DP>
+__global__ void __launch_bounds__(64 * (WA_SINK_NW<T, DP>), 1) wa_bwd_sink_kernel(const WaArgs g)
+{
+    constexpr int PREC = WaT<T>::PB, NP = Mx<PREC>::NP, IMG = NP * 32 * WaImg<DP>::ROWB, ND = DP / 32, NW = (WA_SINK_NW<T, DP>);
+    extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
+    const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    unsigned char *Qimg = at_smem + wv * (2 * IMG + 256), *Gimg = Qimg + IMG;                     // a wave's own images
+    float *Ls = reinterpret_cast<float *>(Gimg + IMG), *Ds = Ls + 32;
+    const int chunk = blockIdx.x % g.nchunk, st = blockIdx.x / g.nchunk % g.nst, bg = blockIdx.x / g.nchunk / g.nst, b = bg / g.G, gi = bg % g.G;
+    const int len = wa_length(g.lengths, b, g.N), k0 = st * 32, ki = k0 + j;
+
+    uint4 kp[DP / 16][NP], vp[DP / 16][NP];
+    wa_colfrags<T, PREC, DP>((const T *)g.k + b * g.ks.b + (long long)ki * g.ks.r + gi * g.ks.h, ki < len, g.D, h, kp);
+    wa_colfrags<T, PREC, DP>((const T *)g.v + b * g.vs.b + (long long)ki * g.vs.r + gi * g.vs.h, ki < len, g.D, h, vp);
+    f32x16 AK[ND], AV[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { AK[d][r] = 0.f; AV[d][r] = 0.f; }
+
+    const int tlo = min(len, k0 + g.left + 1) / 32, per = (len + 31) / 32 - tlo;               // row tiles that hold i > k0 + left
+    const int total = max(per, 0) * g.HG, each = (total + g.nchunk - 1) / g.nchunk, f0 = chunk * each, f1 = min(total, f0 + each);
+    for (int f = f0; f < f1; f += NW) {                                                         // trip count is the workgroup's
+        const int ff = f + wv;
+        const bool on = ff < f1;
+        const int head = gi * g.HG + (on ? ff / per : 0), p0 = on ? (tlo + ff % per) * 32 : 0;
+        if (on) {
+            WaStage<T, DP, 32, 64> sq, sg;
+            sq.load((const T *)g.q + b * g.qs.b + (long long)p0 * g.qs.r + head * g.qs.h, g.qs.r, p0, len, g.D, lane);
+            sg.load((const T *)g.dout + b * g.gs.b + (long long)p0 * g.gs.r + head * g.gs.h, g.gs.r, p0, len, g.D, lane);
+            sq.template put<PREC>(Qimg, lane);
+            sg.template put<PREC>(Gimg, lane);
+            (lane < 32 ? Ls : Ds)[j] = p0 + j < len ? (lane < 32 ? g.lse : g.delta)[((size_t)b * g.H + head) * g.N + p0 + j] : 0.f;
+        }
+        __syncthreads();
+        if (on) wa_dkv_tile<T, PREC, DP, true>(g, Qimg, Gimg, Ls, Ds, p0, k0, len, lane, kp, vp, AK, AV);
+        __syncthreads();
+    }
+    float *sum = reinterpret_cast<float *>(at_smem);                                            // [dK | dV][channel][key]
+    for (int w = 0; w < NW; ++w) {
+        if (wv == w) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float *a = sum + (32 * d + at_drow(r, h)) * 32 + j, *v = a + DP * 32;
+                    *a = w ? *a + AK[d][r] : AK[d][r];
+                    *v = w ? *v + AV[d][r] : AV[d][r];
+                }
+        }
+        __syncthreads();
+    }
+    float *o = g.part + (size_t)blockIdx.x * (2 * DP * 32);
+    for (int e = t; e < 2 * DP * 32; e += 64 * NW) o[e] = sum[e];
+}
+
+// ------------------------------------------------------------------ the last T positions of cached sequences
+// Columns of a wave's tile = up to 32 (head of the key head, row) pairs, so that a cached key is read once for all of them.  The
+// visible key tiles of a sequence are dealt to the waves of its nchunk workgroups in turn; each wave keeps its own running
+// softmax, the waves of a workgroup join through LDS, the workgroups (nchunk > 1) through part[..][m | l | O] and a second kernel.
+template <class T, int DP> constexpr int WA_STEP_NW = sizeof(T) == 4 && DP == 128 ? 4 : 8;
+template <class T, int DP>
+__global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP>), 1) wa_step_kernel(const WaArgs g, T *__restrict__ out)
+{
+    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, IMG = NP * 32 * WaImg<DP>::ROWB, ND = DP / 32, NK = DP / 16, NW = (WA_STEP_NW<T, DP>);
+    extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
+    const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
+    unsigned char *Vimg = at_smem + wv * IMG;
+    const int sp = blockIdx.x % g.nchunk, cb = blockIdx.x / g.nchunk % g.nblk, bg = blockIdx.x / g.nchunk / g.nblk, b = bg / g.G, gi = bg % g.G;
+    const int len = wa_length(g.lengths, b, g.S), col = cb * 32 + j, hs = col / g.N, head = gi * g.HG + hs, tq = col % g.N, qi = len - g.N + tq;
+    const bool mine = hs < g.HG && qi >= 0;
+    const T *kb_ = (const T *)g.k + b * g.ks.b + gi * g.ks.h, *vb = (const T *)g.v + b * g.vs.b + gi * g.vs.h;
+
+    uint4 qp[NK][NP];
+    wa_colfrags<T, PREC, DP>((const T *)g.q + b * g.qs.b + tq * g.qs.r + head * g.qs.h, mine, g.D, h, qp);
+    float m = -__builtin_inff(), mc = 0.f, l = 0.f;
+    f32x16 O[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[d][r] = 0.f;
+
+    const int first = max(0, len - g.N - g.left), tlo = first / 32, thi = (len - 1) / 32;
+    const int nsink = min((min(g.sinks, len) + 31) / 32, tlo), nt = len > 0 ? nsink + thi - tlo + 1 : 0;
+    const float thr = WA_LAZY / g.c;
+    WaRaw<T> rk[NK], rv[NK];                             // lane (row j, half h): channels 16 kb + 8 h ..
+    auto row0 = [&](int tt) { return (tt < nsink ? tt : tlo + tt - nsink) * 32; };
+    auto load = [&](int tt) {
+        const int r0 = row0(tt);
+        const T *kr = kb_ + (long long)(r0 + j) * g.ks.r, *vr = vb + (long long)(r0 + j) * g.vs.r;
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb) {
+            const int ch = 16 * kb + 8 * h;
+            rk[kb] = wa_zero<T>();
+            rv[kb] = wa_zero<T>();
+            if (r0 + j < len && ch < g.D) { rk[kb] = wa_load8<T>(kr + ch); rv[kb] = wa_load8<T>(vr + ch); }
+        }
+    };
+    const int step = NW * g.nchunk;
+    int tt = sp * NW + wv;
+    if (tt < nt) load(tt);
+    for (; tt < nt; tt += step) {
+        const int j0 = row0(tt);
+        f32x16 acc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < NK; ++kb) {
+            uint4 ak[NP], pv[NP];
+            wa_pieces<T, PREC>(rk[kb], ak);
+            mm_mac<PREC>(ak, qp[kb], acc);
+            wa_pieces<T, PREC>(rv[kb], pv);
+#pragma unroll
+            for (int p = 0; p < NP; ++p) *reinterpret_cast<uint4 *>(Vimg + p * WaImg<DP>::template plane<32>() + j * WaImg<DP>::ROWB + 32 * kb + 16 * h) = pv[p];
+        }
+        if (tt + step < nt) load(tt + step);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // the image is the wave's own: LDS serves a wave in order
+        __builtin_amdgcn_wave_barrier();
+        float tmax = -__builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int jj = j0 + at_drow(r, h);
+            const bool ok = jj < len && jj <= qi && (jj >= qi - g.left || jj < g.sinks);
+            acc[r] = ok ? acc[r] : -__builtin_inff();
+            tmax = fmaxf(tmax, acc[r]);
+        }
+        tmax = wa_max32(tmax);
+        if (__ballot(tmax > m + thr) != 0ull) {
+            const float m_new = fmaxf(m, tmax), mc_new = m_new == -__builtin_inff() ? 0.f : m_new * g.c;
+            const float sc = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mc - mc_new);
+            m = m_new;
+            mc = mc_new;
+            l *= sc;
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) O[d][r] *= sc;
+        }
+        float pd[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            pd[r] = __builtin_amdgcn_exp2f(fmaf(acc[r], g.c, -mc));
+            l += pd[r];
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            uint4 pp[NP], av[NP];
+            at_regfrag<PREC>(pd, ks, pp);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                wa_trfrag<PREC, DP, 32>(Vimg, lane, d, ks, av);
+                mm_mac<PREC>(av, pp, O[d]);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    // join the waves: [wave][m, l][32] then [channel][32] sums in wave order
+    l = wa_sum32(l);
+    const float mb = m == -__builtin_inff() ? -__builtin_inff() : mc;      // maximum in base-2 units
+    __syncthreads();
+    float *ml = reinterpret_cast<float *>(at_smem), *osum = ml + NW * 64;
+    if (h == 0) { ml[wv * 64 + j] = mb; ml[wv * 64 + 32 + j] = l; }
+    __syncthreads();
+    float M = -__builtin_inff(), Lt = 0.f;
+    for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w * 64 + j]);
+    for (int w = 0; w < NW; ++w) {
+        const float mw = ml[w * 64 + j];
+        Lt += mw == -__builtin_inff() ? ml[w * 64 + 32 + j] : ml[w * 64 + 32 + j] * __builtin_amdgcn_exp2f(mw - M);
+    }
+    const float f = mb == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(mb - M);      // a wave without keys holds zeros
+    for (int w = 0; w < NW; ++w) {
+        if (wv == w) {
+#pragma unroll
+            for (int d = 0; d < ND; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float *a = osum + (32 * d + at_drow(r, h)) * 32 + j;
+                    *a = w ? fmaf(O[d][r], f, *a) : O[d][r] * f;
+                }
+        }
+        __syncthreads();
+    }
+    if (g.nchunk > 1) {
+        float *o = g.part + (size_t)blockIdx.x * (64 + DP * 32);
+        if (wv == 0 && h == 0) { o[j] = M; o[32 + j] = Lt; }
+        for (int e = t; e < DP * 32; e += 64 * NW) o[64 + e] = osum[e];
+        return;
+    }
+    const float inv = Lt > 0.f ? 1.f / Lt : (Lt != Lt ? Lt : 0.f);
+    if (hs < g.HG)
+        for (int ch = 4 * (t >> 5); ch < g.D; ch += 8 * NW)
+            wa_store4<T>(out + (((size_t)b * g.N + tq) * g.H + head) * g.D + ch, osum[ch * 32 + j] * inv, osum[(ch + 1) * 32 + j] * inv,
+                         osum[(ch + 2) * 32 + j] * inv, osum[(ch + 3) * 32 + j] * inv);
+}
+
+// joins the nchunk partial softmaxes of one (sequence, key head, 32 columns): thread = (column, 4 channels)
+template <class T, int DP>
+__global__ void __launch_bounds__(256) wa_join_kernel(const WaArgs g, T *__restrict__ out)
+{
+    const int t = threadIdx.x, j = t & 31;
+    const int cb = blockIdx.x % g.nblk, bg = blockIdx.x / g.nblk, b = bg / g.G, gi = bg % g.G;
+    const int col = cb * 32 + j, hs = col / g.N, head = gi * g.HG + hs, tq = col % g.N;
+    if (hs >= g.HG) return;
+    const float *pt = g.part + (size_t)blockIdx.x * g.nchunk * (64 + DP * 32);
+    float M = -__builtin_inff(), Lt = 0.f;
+    for (int s = 0; s < g.nchunk; ++s) M = fmaxf(M, pt[(size_t)s * (64 + DP * 32) + j]);
+    for (int ch = 4 * (t >> 5); ch < g.D; ch += 32) {
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+        Lt = 0.f;
+        for (int s = 0; s < g.nchunk; ++s) {
+            const float *p = pt + (size_t)s * (64 + DP * 32), ms = p[j];
+            const float f = ms == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ms - M);
+            Lt = fmaf(p[32 + j], f, Lt);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(p[64 + (ch + e) * 32 + j], f, o[e]);
+        }
+        const float inv = Lt > 0.f ? 1.f / Lt : (Lt != Lt ? Lt : 0.f);
+        wa_store4<T>(out + (((size_t)b * g.N + tq) * g.H + head) * g.D + ch, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    }
+}
+
+// ------------------------------------------------------------------ host side
+int wa_check(const char *who, const gfs3d_window_attn_args *a)
+{
+    GFS3D_REQUIRE(a, "%s: NULL args", who);
+    GFS3D_REQUIRE(a->type == GFS3D_COMPUTE_F32 || a->type == GFS3D_COMPUTE_BF16 || a->type == GFS3D_COMPUTE_F16,
+                  "%s: type must be one of GFS3D_COMPUTE_*", who);
+    GFS3D_REQUIRE(a->B >= 1 && a->N >= 1 && a->S >= 1 && a->S <= (1 << 29) && a->N <= (1 << 29), "%s: bad shape B=%d N=%d S=%d", who, a->B, a->N, a->S);
+    GFS3D_REQUIRE(a->G >= 1 && a->H >= a->G && a->H % a->G == 0, "%s: %d heads over %d key heads", who, a->H, a->G);
+    GFS3D_REQUIRE(a->D >= 8 && a->D <= 128 && a->D % 8 == 0, "%s: head size %d unsupported (a multiple of 8 up to 128)", who, a->D);
+    GFS3D_REQUIRE(a->left >= 0 && a->right >= 0 && a->sinks >= 0, "%s: left=%d right=%d sinks=%d", who, a->left, a->right, a->sinks);
+    GFS3D_REQUIRE(a->scale > 0.f && a->scale < 3e38f, "%s: scale %g must be positive and finite", who, (double)a->scale);
+    GFS3D_REQUIRE(a->q && a->k && a->v && a->out, "%s: NULL buffer", who);
+    const int gran = 16 / (a->type == GFS3D_COMPUTE_F32 ? 4 : 2);
+    const long long *st[4] = {a->q_stride, a->k_stride, a->v_stride, a->dout_stride};
+    const void *pt[4] = {a->q, a->k, a->v, a->dout};
+    for (int n = 0; n < 4; ++n) {
+        if (!pt[n]) continue;
+        GFS3D_REQUIRE(((uintptr_t)pt[n] & 15) == 0, "%s: a tensor is not aligned to 16 bytes", who);
+        for (int e = 0; e < 3; ++e) GFS3D_REQUIRE(st[n][e] >= 0 && st[n][e] % gran == 0, "%s: a stride is negative or not a multiple of 16 bytes", who);
+    }
+    return GFS3D_OK;
+}
+int wa_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
+WaArgs wa_args(const gfs3d_window_attn_args *a)
+{
+    WaArgs g{};
+    g.q = a->q; g.k = a->k; g.v = a->v; g.out = a->out; g.dout = a->dout;
+    g.qs = {a->q_stride[0], a->q_stride[1], a->q_stride[2]};
+    g.ks = {a->k_stride[0], a->k_stride[1], a->k_stride[2]};
+    g.vs = {a->v_stride[0], a->v_stride[1], a->v_stride[2]};
+    g.gs = {a->dout_stride[0], a->dout_stride[1], a->dout_stride[2]};
+    g.lengths = a->lengths; g.lse = a->lse;
+    g.B = a->B; g.N = a->N; g.S = a->S; g.H = a->H; g.G = a->G; g.HG = a->H / a->G; g.D = a->D;
+    g.left = a->left < a->S ? a->left : a->S; g.right = a->right < a->S ? a->right : a->S; g.sinks = a->sinks < a->S ? a->sinks : a->S;
+    g.scale = a->scale; g.c = a->scale * 1.4426950408889634f;
+    return g;
+}
+// the sinks' gradient kernel runs where some row lies beyond the first key's window; at most 32 chunks of at least 8 row tiles
+void wa_sink_plan(WaArgs &g)
+{
+    g.nst = g.sinks > 0 && g.N > g.left + 1 ? (g.sinks + 31) / 32 : 0;
+    const long long tiles = (long long)((g.N + 31) / 32) * g.HG;
+    g.nchunk = (int)(tiles / 8 < 1 ? 1 : tiles / 8 > 32 ? 32 : tiles / 8);
+}
+size_t wa_sink_floats(const WaArgs &g) { return (size_t)g.B * g.G * g.nst * g.nchunk * 2 * wa_dp(g.D) * 32; }
+void wa_step_plan(WaArgs &g)
+{
+    const int NW = 8;
+    g.nblk = (int)(((long long)g.HG * g.N + 31) / 32);
+    const long long keys = (long long)g.left + g.N < g.S ? (long long)g.left + g.N : g.S;
+    const long long tiles = keys / 32 + 2 + (g.sinks + 31) / 32, blocks = (long long)g.B * g.G * g.nblk;
+    long long n = (512 + blocks - 1) / blocks;
+    if (n > tiles / (2 * NW)) n = tiles / (2 * NW);
+    g.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+}
+template <class T, int DP> int wa_forward(WaArgs g, void *out, hipStream_t st, const char *who)
+{
+    constexpr size_t lds = 4ull * Mx<WaT<T>::PF>::NP * WaT<T>::KT * WaImg<DP>::ROWB;
+    g.nblk = (int)(((long long)((g.N + 31) / 32) * g.HG + 3) / 4);
+    const size_t blocks = (size_t)g.B * g.G * g.nblk;
+    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
+    GFS3D_ENSURE_LDS((wa_fwd_kernel<T, DP>), lds, who);
+    hipLaunchKernelGGL((wa_fwd_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), lds, st, g, (T *)out);
+    GFS3D_LAUNCH_CHECK("wa_fwd_kernel");
+    return GFS3D_OK;
+}
+template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *dv, hipStream_t st, const char *who)
+{
+    constexpr int NP = Mx<WaT<T>::PB>::NP;
+    constexpr size_t img = (size_t)NP * 32 * WaImg<DP>::ROWB, lds = 4 * img, ldk = lds + 4 * 32 * sizeof(float);
+    const size_t ub = ((size_t)((g.N + 31) / 32) * g.HG + 3) / 4, kb = ((size_t)g.N + 127) / 128;
+    GFS3D_REQUIRE(ub * g.B * g.G < (1ull << 31), "%s: %zu workgroups", who, ub * g.B * g.G);
+    GFS3D_ENSURE_LDS((wa_bwd_dq_kernel<T, DP>), lds, who);
+    GFS3D_ENSURE_LDS((wa_bwd_dkv_kernel<T, DP>), ldk, who);
+    g.nblk = (int)ub;
+    hipLaunchKernelGGL((wa_bwd_dq_kernel<T, DP>), dim3((unsigned)(ub * g.B * g.G)), dim3(256), lds, st, g, (T *)dq);
+    GFS3D_LAUNCH_CHECK("wa_bwd_dq_kernel");
+    if (g.nst > 0) {
+        constexpr int NW = (WA_SINK_NW<T, DP>);
+        constexpr size_t ws = (size_t)NW * (2 * img + 256), sum = 2ull * DP * 32 * sizeof(float), lsk = ws > sum ? ws : sum;
+        const size_t blocks = (size_t)g.B * g.G * g.nst * g.nchunk;
+        GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
+        GFS3D_ENSURE_LDS((wa_bwd_sink_kernel<T, DP>), lsk, who);
+        hipLaunchKernelGGL((wa_bwd_sink_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lsk, st, g);
+        GFS3D_LAUNCH_CHECK("wa_bwd_sink_kernel");
+    }
+    g.nblk = (int)kb;
+    hipLaunchKernelGGL((wa_bwd_dkv_kernel<T, DP>), dim3((unsigned)(kb * g.B * g.G)), dim3(256), ldk, st, g, (T *)dk, (T *)dv);
+    GFS3D_LAUNCH_CHECK("wa_bwd_dkv_kernel");
+    return GFS3D_OK;
+}
+template <class T, int DP> int wa_step(const WaArgs &g, void *out, hipStream_t st, const char *who)
+{
+    constexpr int NW = (WA_STEP_NW<T, DP>);
+    constexpr size_t im = (size_t)NW * Mx<WaT<T>::PF>::NP * 32 * WaImg<DP>::ROWB, js = (size_t)(NW * 64 + DP * 32) * sizeof(float), lds = im > js ? im : js;
+    const size_t groups = (size_t)g.B * g.G * g.nblk, blocks = groups * g.nchunk;
+    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
+    GFS3D_ENSURE_LDS((wa_step_kernel<T, DP>), lds, who);
+    hipLaunchKernelGGL((wa_step_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)out);
+    GFS3D_LAUNCH_CHECK("wa_step_kernel");
+    if (g.nchunk > 1) {
+        hipLaunchKernelGGL((wa_join_kernel<T, DP>), dim3((unsigned)groups), dim3(256), 0, st, g, (T *)out);
+        GFS3D_LAUNCH_CHECK("wa_join_kernel");
+    }
+    return GFS3D_OK;
+}
+
+// one call per (type, padded head size)
+#define WA_DISPATCH(call)                                                                                                            \
+    switch (wa_dp(a->D) * 4 + a->type) {                                                                                             \
+    case 32 * 4 + GFS3D_COMPUTE_F32: { using T = float; constexpr int DP = 32; return call; }                                        \
+    case 64 * 4 + GFS3D_COMPUTE_F32: { using T = float; constexpr int DP = 64; return call; }                                        \
+    case 128 * 4 + GFS3D_COMPUTE_F32: { using T = float; constexpr int DP = 128; return call; }                                      \
+    case 32 * 4 + GFS3D_COMPUTE_BF16: { using T = __bf16; constexpr int DP = 32; return call; }                                      \
+    case 64 * 4 + GFS3D_COMPUTE_BF16: { using T = __bf16; constexpr int DP = 64; return call; }                                      \
+    case 128 * 4 + GFS3D_COMPUTE_BF16: { using T = __bf16; constexpr int DP = 128; return call; }                                    \
+    case 32 * 4 + GFS3D_COMPUTE_F16: { using T = _Float16; constexpr int DP = 32; return call; }                                     \
+    case 64 * 4 + GFS3D_COMPUTE_F16: { using T = _Float16; constexpr int DP = 64; return call; }                                     \
+    default: { using T = _Float16; constexpr int DP = 128; return call; }                                                            \
+    }
+
+}  // namespace
+}  // namespace gfs3d
+
+extern "C" size_t gfs3d_window_attn_workspace_bytes(int B, int N, int S, int H, int G, int D, int left, int sinks, int step)
+{
+    if (B < 1 || N < 1 || S < 1 || G < 1 || H < G || H % G || D < 8 || D > 128 || left < 0 || sinks < 0) return 0;
+    WaArgs g{};
+    g.B = B; g.N = N; g.S = S; g.H = H; g.G = G; g.HG = H / G; g.D = D;
+    g.left = left < S ? left : S; g.sinks = sinks < S ? sinks : S;
+    if (step) {
+        wa_step_plan(g);
+        return g.nchunk > 1 ? (size_t)B * G * g.nblk * g.nchunk * (64 + wa_dp(D) * 32) * sizeof(float) : 0;
+    }
+    wa_sink_plan(g);
+    return (align_up((size_t)B * H * N, 64) + wa_sink_floats(g)) * sizeof(float);
+}
+
+extern "C" int gfs3d_window_attn_forward(const gfs3d_window_attn_args *a, void *stream)
+{
+    const char *who = "gfs3d_window_attn_forward";
+    if (int rc = wa_check(who, a)) return rc;
+    GFS3D_REQUIRE(a->S == a->N, "%s: S=%d differs from N=%d", who, a->S, a->N);
+    const WaArgs g = wa_args(a);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    WA_DISPATCH((wa_forward<T, DP>(g, a->out, st, who)))
+}
+
+extern "C" int gfs3d_window_attn_backward(const gfs3d_window_attn_args *a, void *stream)
+{
+    const char *who = "gfs3d_window_attn_backward";
+    if (int rc = wa_check(who, a)) return rc;
+    GFS3D_REQUIRE(a->S == a->N, "%s: S=%d differs from N=%d", who, a->S, a->N);
+    GFS3D_REQUIRE(a->lse && a->dout && a->dq && a->dk && a->dv && a->workspace, "%s: NULL buffer", who);
+    WaArgs g = wa_args(a);
+    wa_sink_plan(g);
+    const size_t need = gfs3d_window_attn_workspace_bytes(a->B, a->N, a->S, a->H, a->G, a->D, a->left, a->sinks, 0);
+    if (a->workspace_bytes < need) {
+        set_error("%s: workspace too small (%zu, needs %zu)", who, a->workspace_bytes, need);
+        return GFS3D_ERR_WORKSPACE;
+    }
+    g.delta = (float *)a->workspace;
+    g.part = g.delta + align_up((size_t)a->B * a->H * a->N, 64);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    WA_DISPATCH((wa_backward<T, DP>(g, a->dq, a->dk, a->dv, st, who)))
+}
+
+extern "C" int gfs3d_window_attn_step(const gfs3d_window_attn_args *a, void *stream)
+{
+    const char *who = "gfs3d_window_attn_step";
+    if (int rc = wa_check(who, a)) return rc;
+    GFS3D_REQUIRE(a->lengths, "%s: NULL lengths", who);
+    WaArgs g = wa_args(a);
+    wa_step_plan(g);
+    const size_t need = gfs3d_window_attn_workspace_bytes(a->B, a->N, a->S, a->H, a->G, a->D, a->left, a->sinks, 1);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need)) {
+        set_error("%s: workspace too small (%zu, needs %zu)", who, a->workspace_bytes, need);
+        return GFS3D_ERR_WORKSPACE;
+    }
+    g.part = (float *)a->workspace;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    WA_DISPATCH((wa_step<T, DP>(g, a->out, st, who)))
+}

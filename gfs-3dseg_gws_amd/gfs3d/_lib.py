@@ -154,6 +154,42 @@ class CaplEvalArgs(Structure):
     ]
 
 
+class WindowAttnArgs(Structure):
+    _fields_ = [
+        ("B", c_int), ("N", c_int), ("S", c_int), ("H", c_int), ("G", c_int), ("D", c_int), ("type", c_int),
+        ("left", c_int), ("right", c_int), ("sinks", c_int), ("scale", c_float),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
+        ("q_stride", c_longlong * 3), ("k_stride", c_longlong * 3), ("v_stride", c_longlong * 3),
+        ("lengths", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+        ("dout", c_void_p), ("dout_stride", c_longlong * 3),
+        ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
+class RotaryArgs(Structure):
+    _fields_ = [
+        ("B", c_int), ("N", c_int), ("D", c_int), ("type", c_int), ("q_heads", c_int), ("k_heads", c_int),
+        ("q", c_void_p), ("k", c_void_p), ("q_out", c_void_p), ("k_out", c_void_p),
+        ("q_stride", c_longlong * 3), ("k_stride", c_longlong * 3), ("q_out_stride", c_longlong * 3), ("k_out_stride", c_longlong * 3),
+        ("positions", c_void_p),
+        ("position_type", c_int), ("axes", c_int), ("pairs", c_int), ("interleaved", c_int), ("inverse", c_int),
+        ("freqs", c_void_p), ("magnitude", c_float),
+    ]
+
+
+class RmsNormArgs(Structure):
+    _fields_ = [
+        ("rows", c_longlong),
+        ("C", c_int), ("type", c_int), ("residual_f32", c_int), ("weight_f32", c_int), ("fp8", c_int), ("group", c_int), ("eps", c_float),
+        ("x", c_void_p), ("residual", c_void_p), ("weight", c_void_p), ("x_stride", c_longlong), ("r_stride", c_longlong),
+        ("stream_out", c_void_p), ("y", c_void_p), ("scale", c_void_p), ("rstd", c_void_p),
+        ("dy", c_void_p), ("ds", c_void_p), ("dy_stride", c_longlong), ("ds_stride", c_longlong),
+        ("dx", c_void_p), ("dresidual", c_void_p), ("dweight", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t),
+    ]
+
+
 # every symbol include/gfs3d.h declares: (restype, argtypes)
 SYMBOLS = {
     "gfs3d_version": (c_int, []),
@@ -196,6 +232,14 @@ SYMBOLS = {
                                               c_void_p, c_void_p, c_int, c_void_p]),
     "gfs3d_attention_backward_mixed": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float,
                                                c_float, c_ulonglong, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
+    "gfs3d_window_attn_workspace_bytes": (c_size_t, [c_int] * 9),
+    "gfs3d_window_attn_forward": (c_int, [POINTER(WindowAttnArgs), c_void_p]),
+    "gfs3d_window_attn_backward": (c_int, [POINTER(WindowAttnArgs), c_void_p]),
+    "gfs3d_window_attn_step": (c_int, [POINTER(WindowAttnArgs), c_void_p]),
+    "gfs3d_rotary": (c_int, [POINTER(RotaryArgs), c_void_p]),
+    "gfs3d_rms_norm_workspace_bytes": (c_size_t, [c_longlong, c_int]),
+    "gfs3d_rms_norm_forward": (c_int, [POINTER(RmsNormArgs), c_void_p]),
+    "gfs3d_rms_norm_backward": (c_int, [POINTER(RmsNormArgs), c_void_p]),
     "gfs3d_word_assign_f32": (c_int, [c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_float,
                                       c_void_p, c_void_p, c_void_p, c_void_p]),
     "gfs3d_proto_cosine_f32": (c_int, [c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_int, c_float,
@@ -247,7 +291,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     """Compile every HIP source for gfx950 into lib/libgfs3d_hip.so (hipcc
     cross-compiles without a GPU)."""
     srcs = [os.path.join(_CSRC, s) for s in _SOURCES]
-    deps = srcs + [os.path.join(_CSRC, "common.h"), os.path.join(_PKG, "..", "include", "gfs3d.h")]
+    deps = srcs + [os.path.join(_CSRC, h) for h in ("common.h", "window_attention.h", "row_ops.h")] + [os.path.join(_PKG, "..", "include", "gfs3d.h")]
     if not force and os.path.exists(_SO) and all(os.path.getmtime(_SO) >= os.path.getmtime(d) for d in deps):
         return _SO
     os.makedirs(os.path.dirname(_SO), exist_ok=True)

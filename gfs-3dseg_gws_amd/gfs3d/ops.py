@@ -8,6 +8,7 @@ otherwise - there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -1447,3 +1448,392 @@ class KMeansDelta:
                                                     _stream())
         _lib.check(rc, "gfs3d_kmeans_fix_to_f32")
         return sums, counts
+
+
+# --------------------------------------------------------------------------
+# K7 - K9: a pre-norm attention layer over serialised points (morton.py's order, whole rooms), in fp32, bf16 or half tensors.
+# The arithmetic follows the tensors' type, not set_compute().
+# --------------------------------------------------------------------------
+_TYPE_IDS = {torch.float32: _lib.COMPUTE_F32, torch.bfloat16: _lib.COMPUTE_BF16, torch.float16: _lib.COMPUTE_F16}
+
+
+def _need_typed(who: str, **tensors) -> torch.device:
+    """All given tensors on one GPU and of one supported type."""
+    device = dtype = None
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError(f"gfs3d.{who}: `{name}` must be a HIP (cuda) tensor - the hot path has no CPU fallback")
+        if t.dtype not in _TYPE_IDS:
+            raise RuntimeError(f"gfs3d.{who}: `{name}` must be float32, bfloat16 or float16, got {t.dtype}")
+        if device is None:
+            device, dtype = t.device, t.dtype
+        elif t.device != device or t.dtype != dtype:
+            raise RuntimeError(f"gfs3d.{who}: `{name}` is {t.dtype} on {t.device}, the first tensor {dtype} on {device}")
+    return device
+
+
+def _no_grad_form(who: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"gfs3d.{who} has no backward: call it under torch.no_grad() or on detached tensors")
+
+
+def _launch(fn: str, device: torch.device, args) -> None:
+    call = getattr(_lib.lib(), fn)
+    if device.index == torch.cuda.current_device():
+        rc = call(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = call(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
+    _lib.check(rc, fn)
+
+
+def _heads4(t: torch.Tensor) -> torch.Tensor:
+    """A (B, rows, heads, D) tensor as the attention kernels read it: dense channels, strides and address in 16 bytes; a copy where
+    they are not (one pass over the tensor)."""
+    s, gran = t.stride(), 16 // t.element_size()
+    if s[3] == 1 and s[0] % gran == 0 and s[1] % gran == 0 and s[2] % gran == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _window_args(who, q, k, v, left, right, sinks, scale, lengths):
+    device = _need_typed(who, q=q, k=k, v=v)
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
+        raise RuntimeError(f"gfs3d.{who}: q must be (B, N, H, D), k and v (B, S, G, D), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    B, N, H, D = q.shape
+    S, G = k.shape[1], k.shape[2]
+    if G < 1 or H < 1 or H % G:
+        raise RuntimeError(f"gfs3d.{who}: {H} heads do not divide over {G} key heads")
+    if D < 8 or D > 128 or D % 8:
+        raise NotImplementedError(f"gfs3d.{who}: head sizes are multiples of 8 up to 128, got {D}")
+    if (left is not None and left < 0) or (right is not None and right < 0) or sinks < 0:
+        raise RuntimeError(f"gfs3d.{who}: left, right and sinks must not be negative")
+    scale = 1.0 / D ** 0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 3e38:
+        raise RuntimeError(f"gfs3d.{who}: scale must be positive and finite, got {scale}")
+    if lengths is not None:
+        if not isinstance(lengths, torch.Tensor) or lengths.device != device or lengths.dtype not in (torch.int32, torch.int64) \
+                or tuple(lengths.shape) != (B,):
+            raise RuntimeError(f"gfs3d.{who}: lengths must be an int32 or int64 tensor of shape ({B},) on {device}")
+        if lengths.dtype == torch.int64:
+            lengths = lengths.clamp(0, S).to(torch.int32)
+        lengths = lengths.contiguous()
+    a = _lib.WindowAttnArgs()
+    a.B, a.N, a.S, a.H, a.G, a.D, a.type = B, N, S, H, G, D, _TYPE_IDS[q.dtype]
+    a.left = S if left is None else min(int(left), S)
+    a.right = S if right is None else min(int(right), S)
+    a.sinks, a.scale = min(int(sinks), S), scale
+    a.lengths = lengths.data_ptr() if lengths is not None else None
+    return a, lengths
+
+
+def _window_inputs(a, q, k, v):
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        setattr(a, name, t.data_ptr())
+        s = t.stride()
+        setattr(a, name + "_stride", (ctypes.c_longlong * 3)(s[0], s[1], s[2]))
+
+
+class WindowAttentionFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, left, right, sinks, scale, lengths):
+        a, lengths = _window_args("window_attention", q, k, v, left, right, sinks, scale, lengths)
+        if a.S != a.N:
+            raise RuntimeError(f"gfs3d.window_attention: q has {a.N} rows, k and v {a.S} (the last rows of a cache: window_attention_step)")
+        q, k, v = _heads4(q), _heads4(k), _heads4(v)
+        out = torch.empty((a.B, a.N, a.H, a.D), dtype=q.dtype, device=q.device)
+        grad = any(ctx.needs_input_grad[:3])
+        lse = torch.empty((a.B, a.H, a.N), dtype=torch.float32, device=q.device) if grad else None
+        if out.numel():
+            _window_inputs(a, q, k, v)
+            a.out, a.lse = out.data_ptr(), lse.data_ptr() if grad else None
+            _launch("gfs3d_window_attn_forward", q.device, a)
+        if grad:
+            ctx.save_for_backward(q, k, v, out, lse, lengths)
+            ctx.cfg = (left, right, sinks, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse, lengths = ctx.saved_tensors
+        a, _ = _window_args("window_attention", q, k, v, *ctx.cfg, lengths)
+        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        if out.numel():
+            dout = _heads4(dout)
+            _window_inputs(a, q, k, v)
+            a.out, a.lse, a.dout, a.dq, a.dk, a.dv = (t.data_ptr() for t in (out, lse, dout, dq, dk, dv))
+            s = dout.stride()
+            a.dout_stride = (ctypes.c_longlong * 3)(s[0], s[1], s[2])
+            nbytes = _lib.lib().gfs3d_window_attn_workspace_bytes(a.B, a.N, a.S, a.H, a.G, a.D, a.left, a.sinks, 0)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # from torch's allocator: a captured graph keeps its own
+            a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+            _launch("gfs3d_window_attn_backward", q.device, a)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def window_attention(q, k, v, left: Optional[int] = None, right: Optional[int] = None, sinks: int = 0,
+                     lengths: Optional[torch.Tensor] = None, scale: Optional[float] = None) -> torch.Tensor:
+    """Softmax attention of serialised points in which row i sees the rows j of its sequence with i - left <= j <= i + right, and
+    the first `sinks` rows as far as j <= i + right.  q (B, N, H, D), k / v (B, N, G, D) -> (B, N, H, D); head h reads key head
+    h // (H // G).  left / right None: unlimited (right = 0: causal).  `lengths` (B,): valid rows of each sequence; what lies behind
+    is not read, its outputs and gradients are zero.  Keys and values in front of it have to be finite: a row next to a window takes
+    part in products with zero weights.  scale defaults to D ** -0.5.  fp32, bf16 or half; D a multiple of 8 up to 128.
+    Differentiable once, deterministic."""
+    return WindowAttentionFunction.apply(q, k, v, left, right, int(sinks), scale, lengths)
+
+
+def window_attention_step(q, k, v, lengths, left: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:
+    """window_attention (right = 0) for the last T rows of sequences whose keys and values are cached: q (B, T, H, D), k / v (B, S, G,
+    D) with room for S rows, `lengths` (B,) the sequences' lengths with these T rows (a device tensor: no host read).  Row t stands at
+    position length - T + t; rows in front of the first position are zero.  No backward."""
+    _no_grad_form("window_attention_step", q, k, v)
+    if lengths is None:
+        raise RuntimeError("gfs3d.window_attention_step: lengths (B,) is needed")
+    a, lengths = _window_args("window_attention_step", q, k, v, left, 0, sinks, scale, lengths)
+    out = torch.empty((a.B, a.N, a.H, a.D), dtype=q.dtype, device=q.device)
+    if out.numel() == 0 or a.S == 0:
+        return out.zero_()
+    q, k, v = _heads4(q), _heads4(k), _heads4(v)
+    _window_inputs(a, q, k, v)
+    a.out = out.data_ptr()
+    nbytes = _lib.lib().gfs3d_window_attn_workspace_bytes(a.B, a.N, a.S, a.H, a.G, a.D, a.left, a.sinks, 1)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    a.workspace, a.workspace_bytes = (ws.data_ptr(), nbytes) if nbytes else (None, 0)
+    _launch("gfs3d_window_attn_step", q.device, a)
+    return out
+
+
+_POSITION_IDS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def rotary_frequencies(pairs: int, base: float = 10000.0, scaling: Optional[str] = None, factor: float = 1.0,
+                       original_length: Optional[float] = None, fast: float = 32.0, slow: float = 1.0, device=None):
+    """(freqs, magnitude) for `rotary`: radians per position base ** (-p / pairs) in float64, slowed by `factor` for positions past
+    the length they were trained on.  scaling None; "linear": every pair by the factor; "base": the base raised so that the slowest
+    pair is slowed by the factor and the fastest not at all; "parts": pairs that turn at most `slow` times over `original_length`
+    by the factor, those that turn at least `fast` times not at all, a ramp over the pairs between, and the rotated values times
+    magnitude = 0.1 ln(factor) + 1."""
+    if pairs < 1 or not base > 1.0 or not factor >= 1.0:
+        raise ValueError(f"gfs3d.rotary_frequencies: pairs={pairs} (>= 1), base={base} (> 1), factor={factor} (>= 1)")
+    p = torch.arange(pairs, dtype=torch.float64)
+    magnitude = 1.0
+    if scaling == "base" and pairs > 1:
+        base = base * factor ** (pairs / (pairs - 1.0))
+    freqs = base ** (-p / pairs)
+    if scaling == "linear":
+        freqs = freqs / factor
+    elif scaling == "parts":
+        if original_length is None or not original_length > 0 or not fast > slow > 0:
+            raise ValueError("gfs3d.rotary_frequencies: \"parts\" needs original_length > 0 and fast > slow > 0")
+        lo, hi = (pairs * math.log(original_length / (turns * 2 * math.pi)) / math.log(base) for turns in (fast, slow))
+        lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), pairs - 1)
+        ramp = ((p - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        freqs = freqs / factor * ramp + freqs * (1 - ramp)
+        magnitude = 0.1 * math.log(factor) + 1.0
+    elif scaling not in (None, "base"):
+        raise ValueError(f"gfs3d.rotary_frequencies: scaling must be None, \"linear\", \"base\" or \"parts\", got {scaling!r}")
+    return freqs.to(device) if device is not None else freqs, magnitude
+
+
+def _rotary_launch(q, k, positions, freqs, magnitude, interleaved, inverse):
+    a = _lib.RotaryArgs()
+    B, N, H, D = q.shape
+    a.B, a.N, a.D, a.type = B, N, D, _TYPE_IDS[q.dtype]
+    outs = []
+    for name, t in (("q", q), ("k", k)):
+        if t is None:
+            outs.append(None)
+            continue
+        if t.stride(3) != 1:
+            t = t.contiguous()
+        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        setattr(a, name, t.data_ptr())
+        setattr(a, name + "_out", o.data_ptr())
+        setattr(a, name + "_heads", t.shape[2])
+        s = t.stride()
+        setattr(a, name + "_stride", (ctypes.c_longlong * 3)(s[0], s[1], s[2]))
+        s = o.stride()
+        setattr(a, name + "_out_stride", (ctypes.c_longlong * 3)(s[0], s[1], s[2]))
+        outs.append((o, t))                                   # t: kept until the launch
+    a.positions, a.position_type, a.axes = positions.data_ptr(), _POSITION_IDS[positions.dtype], positions.shape[2]
+    a.pairs, a.interleaved, a.inverse = freqs.numel(), interleaved, inverse
+    a.freqs, a.magnitude = freqs.data_ptr(), magnitude
+    if B and N:
+        _launch("gfs3d_rotary", q.device, a)
+    return tuple(o[0] if o is not None else None for o in outs)
+
+
+class RotaryFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, freqs, magnitude, interleaved):
+        ctx.set_materialize_grads(False)
+        if any(ctx.needs_input_grad[:2]):
+            ctx.save_for_backward(positions, freqs)
+            ctx.cfg = (magnitude, interleaved)
+        return _rotary_launch(q, k, positions, freqs, magnitude, interleaved, 0)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk):
+        positions, freqs = ctx.saved_tensors
+        if dq is None and dk is None:
+            return (None,) * 6
+        if dq is None:
+            gk, gq = _rotary_launch(dk, None, positions, freqs, *ctx.cfg, 1)
+        else:
+            gq, gk = _rotary_launch(dq, dk, positions, freqs, *ctx.cfg, 1)
+        return gq, gk, None, None, None, None
+
+
+def rotary(q, k, positions, freqs, magnitude: float = 1.0, layout: str = "half"):
+    """Rotary positions of q (B, N, H, D) and, if not None, k (B, N, G, D), in one launch: section a of each head, 2 P = 2 len(freqs)
+    channels, turns by the angle positions[.., a] freqs[p] and is multiplied by `magnitude`; channels behind the sections are
+    copied.  layout "half": pair p is the section's channels (p, P + p); "interleaved": (2 p, 2 p + 1).  positions (N,), (B, N) or
+    (B, N, axes) with 1 to 3 axes (a point's coordinates, say), int32, int64 or float32; freqs (P,) float64 on the device
+    (`rotary_frequencies`); angles are formed in float64.  Differentiable in q and k.  Returns (q', k'), or q' alone without k."""
+    device = _need_typed("rotary", q=q, **({"k": k} if k is not None else {}))
+    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+        raise RuntimeError("gfs3d.rotary: q must be (B, N, H, D) and k (B, N, G, D)")
+    if layout not in ("half", "interleaved"):
+        raise ValueError(f"gfs3d.rotary: layout must be \"half\" or \"interleaved\", got {layout!r}")
+    B, N, H, D = q.shape
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_IDS or positions.device != device:
+        raise RuntimeError(f"gfs3d.rotary: positions must be an int32, int64 or float32 tensor on {device}")
+    if positions.dim() == 1:
+        positions = positions.expand(B, positions.shape[0])
+    if positions.dim() == 2:
+        positions = positions[:, :, None]
+    if positions.dim() != 3 or tuple(positions.shape[:2]) != (B, N) or not 1 <= positions.shape[2] <= 3:
+        raise RuntimeError(f"gfs3d.rotary: positions must be ({N},), ({B}, {N}) or ({B}, {N}, 1..3), got {tuple(positions.shape)}")
+    if not isinstance(freqs, torch.Tensor) or freqs.dtype != torch.float64 or freqs.device != device or freqs.dim() != 1:
+        raise RuntimeError(f"gfs3d.rotary: freqs must be a 1-d float64 tensor on {device}")
+    P = freqs.numel()
+    if P < 1 or 2 * P * positions.shape[2] > D or P * positions.shape[2] > 1024 or H < 1 or (k is not None and k.shape[2] < 1):
+        raise RuntimeError(f"gfs3d.rotary: {positions.shape[2]} axes of {P} pairs do not fit heads of {D} channels")
+    positions, freqs = positions.contiguous(), freqs.contiguous()
+    interleaved = 1 if layout == "interleaved" else 0
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        got = RotaryFunction.apply(q, k, positions, freqs, float(magnitude), interleaved)
+    else:
+        got = _rotary_launch(q, k, positions, freqs, float(magnitude), interleaved, 0)
+    return got if k is not None else got[0]
+
+
+def _rows2(t: torch.Tensor) -> torch.Tensor:
+    """(.., C) as (rows, C) with dense channels; a copy only where the rows have no common stride."""
+    C = t.shape[-1]
+    if t.stride(-1) != 1 and C > 1:
+        t = t.contiguous()
+    return t.reshape(-1, C)
+
+
+def _rms_args(who, x, weight, eps, residual):
+    device = _need_typed(who, x=x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"gfs3d.{who}: x must be (.., C)")
+    C = x.shape[-1]
+    if C > 16384:
+        raise NotImplementedError(f"gfs3d.{who}: rows of up to 16384 channels, got {C}")
+    if not isinstance(weight, torch.Tensor) or weight.device != device or weight.dtype not in (torch.float32, x.dtype) or tuple(weight.shape) != (C,):
+        raise RuntimeError(f"gfs3d.{who}: weight must be a ({C},) tensor of float32 or {x.dtype} on {device}")
+    if residual is not None and (not isinstance(residual, torch.Tensor) or residual.device != device or residual.shape != x.shape
+                                 or residual.dtype not in (torch.float32, x.dtype)):
+        raise RuntimeError(f"gfs3d.{who}: residual must have x's shape {tuple(x.shape)}, in float32 or {x.dtype}, on {device}")
+    if not 0.0 <= eps < 3e38:
+        raise RuntimeError(f"gfs3d.{who}: eps must not be negative, got {eps}")
+    a = _lib.RmsNormArgs()
+    a.rows, a.C, a.type = x.numel() // C, C, _TYPE_IDS[x.dtype]
+    a.residual_f32 = int(residual is not None and residual.dtype == torch.float32)
+    a.weight_f32 = int(weight.dtype == torch.float32)
+    a.eps, a.weight = float(eps), weight.data_ptr()
+    return a
+
+
+def _rms_forward(who, x, weight, eps, residual, want_rstd=False, fp8=False, group=0):
+    """(y, scale or None, stream or None, rstd or None, the (rows, C) stream or x that the backward reads)."""
+    weight = weight.contiguous()
+    a = _rms_args(who, x, weight, eps, residual)
+    x2 = _rows2(x)
+    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=x.device)
+    stream = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if residual is not None else None
+    rstd = torch.empty(a.rows, dtype=torch.float32, device=x.device) if want_rstd else None
+    scale = torch.empty(x.shape[:-1] + ((a.C // group,) if group else ()), dtype=torch.float32, device=x.device) if fp8 else None
+    if a.rows:
+        a.x, a.x_stride, a.y = x2.data_ptr(), x2.stride(0), y.data_ptr()
+        if residual is not None:
+            r2 = _rows2(residual)
+            a.residual, a.r_stride, a.stream_out = r2.data_ptr(), r2.stride(0), stream.data_ptr()
+        a.rstd = rstd.data_ptr() if want_rstd else None
+        a.fp8, a.group, a.scale = int(fp8), group, scale.data_ptr() if fp8 else None
+        _launch("gfs3d_rms_norm_forward", x.device, a)
+    return y, scale, stream, rstd, x2
+
+
+class RmsNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        ctx.set_materialize_grads(False)
+        y, _, stream, rstd, x2 = _rms_forward("rms_norm", x, weight, eps, residual, want_rstd=True)
+        ctx.save_for_backward(x2 if stream is None else stream, weight, rstd)
+        ctx.cfg = (x.dtype, float(eps), residual is not None)
+        return y if stream is None else (y, stream)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, ds=None):
+        s, weight, rstd = ctx.saved_tensors
+        dtype, eps, has_res = ctx.cfg
+        shape = dy.shape if dy is not None else ds.shape if ds is not None else None
+        if shape is None:
+            return None, None, None, None
+        need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        if dy is None:
+            return ds.to(dtype) if need_x else None, torch.zeros_like(weight) if need_w else None, ds if need_r else None, None
+        weight = weight.contiguous()
+        s2, dy2 = _rows2(s), _rows2(dy)
+        a = _lib.RmsNormArgs()
+        a.rows, a.C, a.type, a.eps = s2.shape[0], s2.shape[1], _TYPE_IDS[dtype], eps
+        a.residual_f32, a.weight_f32 = int(s.dtype == torch.float32), int(weight.dtype == torch.float32)
+        wide = has_res and s.dtype != dtype                         # an fp32 stream beside 16-bit x: two gradients
+        dx = torch.empty(shape, dtype=dtype, device=s.device) if need_x or (need_r and not wide) else None
+        dr = torch.empty(shape, dtype=s.dtype, device=s.device) if need_r and wide else None
+        dw = torch.empty_like(weight) if need_w else None
+        if a.rows:
+            a.x, a.x_stride, a.weight, a.rstd = s2.data_ptr(), s2.stride(0), weight.data_ptr(), rstd.data_ptr()
+            a.dy, a.dy_stride = dy2.data_ptr(), dy2.stride(0)
+            if ds is not None:
+                ds2 = _rows2(ds)
+                a.ds, a.ds_stride = ds2.data_ptr(), ds2.stride(0)
+            a.dx = dx.data_ptr() if dx is not None else None
+            a.dresidual = dr.data_ptr() if dr is not None else None
+            if need_w:
+                nbytes = _lib.lib().gfs3d_rms_norm_workspace_bytes(a.rows, a.C)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
+                a.dweight, a.workspace, a.workspace_bytes = dw.data_ptr(), ws.data_ptr(), nbytes
+            _launch("gfs3d_rms_norm_backward", s.device, a)
+        elif need_w:
+            dw.zero_()
+        return dx if need_x else None, dw, (dr if wide else dx) if need_r else None, None
+
+
+def rms_norm(x, weight, eps: float = 1e-6, residual: Optional[torch.Tensor] = None):
+    """Root-mean-square norm of the rows of x (.., C):  y = s (mean s^2 + eps)^-1/2 weight  with s = x, or with `residual`
+    s = x + residual rounded to the residual's type (the residual stream; float32 beside 16-bit x is allowed), which is returned
+    too: (y, s).  The statistics are those of s as it is stored, in fp32.  weight (C,) float32 or x's type; C up to 16384.
+    Differentiable once in x, weight and residual, deterministic."""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        return RmsNormFunction.apply(x, weight, residual, float(eps))
+    y, _, stream, _, _ = _rms_forward("rms_norm", x, weight, eps, residual)
+    return y if stream is None else (y, stream)
+
+
+def rms_norm_fp8(x, weight, eps: float = 1e-6, residual: Optional[torch.Tensor] = None, group: Optional[int] = None):
+    """rms_norm with an 8-bit output for a scaled 8-bit product: (q, scale) or, with `residual`, (q, scale, s);  q (.., C)
+    float8_e4m3fn with value = q scale, scale float32 = max(max |value|, 1e-12) / 448 over the row (.., ) or, with group 32, 64 or 128,
+    over every `group` channels (.., C / group).  The values are rounded once, from fp32.  No backward."""
+    _no_grad_form("rms_norm_fp8", x, weight, residual)
+    if group is not None and (group not in (32, 64, 128) or x.shape[-1] % group):
+        raise RuntimeError(f"gfs3d.rms_norm_fp8: group must be 32, 64 or 128 and divide C = {x.shape[-1]}, got {group}")
+    y, scale, stream, _, _ = _rms_forward("rms_norm_fp8", x, weight, eps, residual, fp8=True, group=int(group or 0))
+    return (y, scale) if stream is None else (y, scale, stream)

@@ -348,6 +348,92 @@ int gfs3d_attention_backward_mixed(const float *q, const float *k, const float *
                                    const uint8_t *keep_mask, float *dq, float *dk, float *dv, float *workspace, int compute,
                                    void *stream);
 
+/* ------------------------------------------------------------------ K7 --
+ * Attention with a sliding window and a few first tokens that stay visible, over serialised points (no counterpart in the
+ * reference, whose attention is the full one of K5 over a block):
+ *     out_i = sum_j p_ij v_j,  p_i. = softmax over the visible j of  scale q_i . k_j
+ *     j visible to i:  i, j < length  and  j <= i + right  and  (j >= i - left  or  j < sinks)
+ * Rows that see nothing (those at or behind their sequence's length among them) are zero, and so are their gradients; what lies
+ * behind a sequence's length is not read.
+ *   q (B, N, H, D), k / v (B, S, G, D): any strides (sequence, row, head; in elements, multiples of 16 bytes, >= 0) with dense
+ *   channels, 16-byte aligned; head h reads key head h / (H / G).  D a multiple of 8 up to 128.  out, dq (B, N, H, D) and dk, dv
+ *   (B, N, G, D) are dense.  type: element type of all of them, named as the GFS3D_COMPUTE_* ids (the arithmetic follows it: fp32 at
+ *   fp32 accuracy; bf16 and half products with fp32 scores, statistics and accumulators, gradients of half tensors on two bf16 pieces).
+ *   lengths: (B) device int32 (clamped to 0..S), or NULL = S.  left / right at or above S: unlimited.  scale > 0.
+ * forward (S == N): row i stands at position i.  lse (B, H, N) is written if not NULL: log2 of the sum of 2^(scaled scores
+ *   log2 e), +inf for rows that see nothing (what the backward reads).
+ * backward: dout -> dq, dk, dv; reads q, k, v, out, lse; deterministic (no atomics).
+ * step: the N rows are the last positions of each sequence, row t at length - N + t; right is taken as 0 (S keys of capacity).
+ * Workspace (device, 16-byte aligned): gfs3d_window_attn_workspace_bytes(..., step); 0 for the forward. */
+typedef struct gfs3d_window_attn_args {
+    int B, N, S, H, G, D, type;
+    int left, right, sinks;
+    float scale;
+    const void *q, *k, *v;
+    long long q_stride[3], k_stride[3], v_stride[3];
+    const int *lengths;
+    void *out;
+    float *lse;
+    const void *dout;
+    long long dout_stride[3];
+    void *dq, *dk, *dv;
+    void *workspace;
+    size_t workspace_bytes;
+} gfs3d_window_attn_args;
+size_t gfs3d_window_attn_workspace_bytes(int B, int N, int S, int H, int G, int D, int left, int sinks, int step);
+int gfs3d_window_attn_forward(const gfs3d_window_attn_args *a, void *stream);
+int gfs3d_window_attn_backward(const gfs3d_window_attn_args *a, void *stream);
+int gfs3d_window_attn_step(const gfs3d_window_attn_args *a, void *stream);
+
+/* ------------------------------------------------------------------ K8 --
+ * Rotary positions.  Section a of a head (2 pairs channels; axes sections one behind the other, the channels behind them are copied)
+ * turns by the angle positions[.., a] freqs[p]:  (x, y) -> magnitude (x cos - y sin, y cos + x sin)  over the channel pairs
+ * (p, p + pairs) of the section, or (2 p, 2 p + 1) if interleaved.  inverse turns the other way (the adjoint).
+ *   q (B, N, q_heads, D) and optionally k (B, N, k_heads, D) of the given type, strides as above (any alignment); outputs likewise,
+ *   and may be the inputs themselves.  positions (B, N, axes) dense: position_type 0 int32, 1 int64, 2 fp32.  freqs (pairs) fp64, radians
+ *   per position; angles are formed and reduced in fp64.  1 <= axes <= 3, axes pairs <= 1024, 2 axes pairs <= D. */
+typedef struct gfs3d_rotary_args {
+    int B, N, D, type;
+    int q_heads, k_heads;
+    const void *q, *k;
+    void *q_out, *k_out;
+    long long q_stride[3], k_stride[3], q_out_stride[3], k_out_stride[3];
+    const void *positions;
+    int position_type, axes, pairs, interleaved, inverse;
+    const double *freqs;
+    float magnitude;
+} gfs3d_rotary_args;
+int gfs3d_rotary(const gfs3d_rotary_args *a, void *stream);
+
+/* ------------------------------------------------------------------ K9 --
+ * Root-mean-square norm of rows with the residual's addition:  s = round(x + residual) (to the residual's type; s = x without one),
+ * y = s (mean s^2 + eps)^-1/2 weight.  Statistics are fp32 and of s as it is stored.
+ *   x (rows, C) of the given type, rows x_stride elements apart, 1 <= C <= 16384; residual of the same type or fp32 (residual_f32), rows
+ *   r_stride apart; weight (C) of the same type or fp32 (weight_f32).  stream_out (with a residual) and y are dense; rstd (rows) is
+ *   written if not NULL (the backward reads it).
+ *   fp8: y is e4m3 (OCP) bytes, y = round(value / scale) with scale = max(max |value|, 1e-12) / 448 over the row (group 0: scale
+ *   (rows)) or over every `group` channels (32, 64 or 128, a divisor of C: scale (rows, C / group)).  A NaN makes its group's scale NaN.
+ * backward: x is s (type: the residual's) with x_stride; dy (rows, C), ds (gradient of s in its type; may be NULL) ->
+ *   dx in x's type and, for an fp32 residual beside 16-bit x, dresidual fp32 (otherwise the residual's gradient is dx), dense, each may be
+ *   NULL; dweight in the weight's type if not NULL (deterministic: per-workgroup sums, then a fixed order), with workspace. */
+typedef struct gfs3d_rms_norm_args {
+    long long rows;
+    int C, type, residual_f32, weight_f32, fp8, group;
+    float eps;
+    const void *x, *residual, *weight;
+    long long x_stride, r_stride;
+    void *stream_out, *y;
+    float *scale, *rstd;
+    const void *dy, *ds;
+    long long dy_stride, ds_stride;
+    void *dx, *dresidual, *dweight;
+    void *workspace;
+    size_t workspace_bytes;
+} gfs3d_rms_norm_args;
+size_t gfs3d_rms_norm_workspace_bytes(long long rows, int C);
+int gfs3d_rms_norm_forward(const gfs3d_rms_norm_args *a, void *stream);
+int gfs3d_rms_norm_backward(const gfs3d_rms_norm_args *a, void *stream);
+
 /* ------------------------------------------------------------------ K3 --
  * Point x prototype cosine matching on MFMA (fp32-in / fp32-acc).
  *

@@ -1,0 +1,400 @@
+"""GPU parity of the operators over serialised points (K7 - K9) against plain float64 forms, with derived elementwise bounds."""
+import math
+
+import pytest
+import torch
+
+import serial_oracle as O
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def ops():
+    from gfs3d import ops as o
+    return o
+
+
+def rnd(seed, shape, dtype, mul=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * mul).to(dtype).cuda()
+
+
+# B, N, H, G, D, left, right, sinks, lengths
+ATTEND = [
+    (1, 1, 1, 1, 64, None, None, 0, None),
+    (2, 33, 2, 1, 32, None, 0, 0, None),
+    (1, 64, 1, 1, 64, 0, 0, 0, None),                       # a row sees itself alone
+    (2, 130, 4, 2, 64, 7, 3, 0, None),
+    (1, 257, 3, 1, 40, 50, 0, 5, None),
+    (2, 200, 6, 2, 128, 31, 32, 33, [200, 77]),
+    (3, 161, 2, 2, 16, 20, 0, 64, [0, 1, 161]),             # an empty sequence, one of one row
+    (1, 300, 5, 5, 8, 64, 64, 1, [299]),
+    (2, 96, 8, 1, 96, None, None, 0, [96, 50]),
+    (1, 520, 1, 1, 64, 100, 60, 70, None),
+    (1, 1100, 2, 1, 48, 33, 0, 3, [1090]),                  # several chunks of sink rows
+    (1, 128, 1, 1, 80, 1000, 1000, 200, None),              # everything behind the sequence's ends
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(ATTEND)))
+def test_window_attention_forward_and_gradients(case, dtype):
+    B, N, H, G, D, left, right, sinks, lens = ATTEND[case]
+    q, k, v = rnd(1, (B, N, H, D), dtype), rnd(2, (B, N, G, D), dtype), rnd(3, (B, N, G, D), dtype)
+    g = rnd(4, (B, N, H, D), dtype)
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for t in (q, k, v):
+        t.requires_grad_()
+    out = ops().window_attention(q, k, v, left=left, right=right, sinks=sinks, lengths=lengths)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    want = O.attention(q, k, v, left, right, sinks, lens, dout=g, dtype=dtype)
+    for name, x in zip(("out", "dq", "dk", "dv"), (out,) + grads):
+        O.check(f"{name} {dtype} {ATTEND[case]}", x, want[name])
+    with torch.no_grad():                                   # the form that keeps nothing for a backward
+        assert torch.equal(ops().window_attention(q, k, v, left=left, right=right, sinks=sinks, lengths=lengths), out)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_window_attention_reads_nothing_behind_a_sequence(dtype):
+    """NaN and infinities behind the lengths, in every input, change nothing; rows there are zero."""
+    B, N, H, G, D = 2, 150, 4, 2, 64
+    lens = torch.tensor([90, 150], device="cuda")            # int64 lengths
+    base = [rnd(5, (B, N, H, D), dtype), rnd(6, (B, N, G, D), dtype), rnd(7, (B, N, G, D), dtype), rnd(8, (B, N, H, D), dtype)]
+    dirty = [t.clone() for t in base]
+    for n, t in enumerate(dirty):
+        t[0, 90:] = (math.nan, math.inf, -math.inf, math.nan)[n]
+    got = []
+    for q, k, v, g in (base, dirty):
+        q, k, v = (t.clone().requires_grad_() for t in (q, k, v))
+        out = ops().window_attention(q, k, v, left=40, right=10, sinks=3, lengths=lens)
+        got.append((out.detach(),) + torch.autograd.grad(out, (q, k, v), g))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+        assert not a[0, 90:].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_window_attention_large_and_equal_scores(dtype):
+    """Scores of +-300 (the maximum moves far between tiles) and rows whose scores are all equal."""
+    N, D = 200, 64
+    q, k, v = rnd(9, (1, N, 1, D), dtype, 6.0), rnd(10, (1, N, 1, D), dtype, 6.0), rnd(11, (1, N, 1, D), dtype)
+    q[0, 100:] = 0
+    out = ops().window_attention(q, k, v, left=150, right=0)
+    want = O.attention(q, k, v, 150, 0, 0, None, dtype=dtype)
+    O.check("out", out, want["out"])
+    O.check("mean", out[:, 150:151], (v[:, :151].double().cpu().mean(1, keepdim=True), O.attention(q, k, v, 150, 0, 0, None, dtype=dtype)["out"][1][:, 150:151]))
+
+
+def test_window_attention_strides_and_copies():
+    """Channel slices of one projection, transposed heads, an expanded gradient, an unaligned view (copied), against dense inputs."""
+    B, N, H, D = 2, 70, 2, 64
+    for dtype in TYPES:
+        packed = rnd(12, (B, N, 3, H, D), dtype)
+        q, k, v = packed.unbind(2)
+        dense = [t.contiguous() for t in (q, k, v)]
+        want = ops().window_attention(*dense, left=9, right=9, sinks=2)
+        assert torch.equal(ops().window_attention(q, k, v, left=9, right=9, sinks=2), want)
+        swapped = [t.transpose(1, 2).contiguous().transpose(1, 2) for t in dense]
+        assert torch.equal(ops().window_attention(*swapped, left=9, right=9, sinks=2), want)
+        odd = torch.empty(B * N * H * D + 1, dtype=dtype, device="cuda")[1:].view(B, N, H, D)
+        odd.copy_(q)
+        assert torch.equal(ops().window_attention(odd, k, v, left=9, right=9, sinks=2), want)
+        grads = []
+        for ins in (dense, swapped):
+            ins = [t.detach().requires_grad_() for t in ins]
+            out = ops().window_attention(*ins, left=9, right=9, sinks=2)
+            grads.append(torch.autograd.grad(out, ins, torch.ones((), dtype=dtype, device="cuda").expand_as(out)))
+        assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_window_attention_gradient_against_differences():
+    """The directional derivative of sum(w o) in fp32: central differences of step h are off by h^2 f'''/6 and 2 u32 |f| / h."""
+    B, N, H, G, D = 1, 90, 2, 1, 32
+    q, k, v, w = (rnd(n, (B, N, h, D), torch.float32) for n, h in ((13, H), (14, G), (15, G), (16, H)))
+    ins = [t.requires_grad_() for t in (q, k, v)]
+    f = lambda *a: float((ops().window_attention(*a, left=20, right=5, sinks=4).double() * w.double()).sum())  # noqa: E731
+    grads = torch.autograd.grad(ops().window_attention(*ins, left=20, right=5, sinks=4), ins, w)
+    for n in range(3):
+        d = rnd(17 + n, ins[n].shape, torch.float32)
+        d /= d.norm()
+        h = 2.0 ** -6
+        with torch.no_grad():
+            moved = [[t + s * h * d if m == n else t for m, t in enumerate(ins)] for s in (1, -1)]
+            slope = (f(*moved[0]) - f(*moved[1])) / (2 * h)
+        at = float((grads[n].double() * d.double()).sum())
+        # f is a sum of B N H D weighted means: its rounding noise is about u32 sqrt(B N H D) |w o|, far below the bound; f''' of a
+        # softmax along a unit direction is below 8 |w| |v|, here about 8 * 8 * 8
+        assert abs(slope - at) <= h * h * 512 / 6 + 1e-3, (n, slope, at)
+
+
+def test_window_attention_offsets_past_32_bits():
+    """A view whose rows and sequences lie more than 2^32 elements into its storage."""
+    free = torch.cuda.mem_get_info()[0]
+    need = 2 * (2 ** 32 + 2 ** 22)
+    if free < 2 * need:
+        pytest.skip("needs 17 GB of free memory")
+    store = torch.empty(2 ** 32 + 2 ** 22, dtype=torch.bfloat16, device="cuda")
+    B, N, H, D = 2, 40, 1, 64
+    view = lambda off: torch.as_strided(store, (B, N, H, D), (2 ** 32, 256, 64, 1), off)  # noqa: E731
+    q, k, v = (view(off) for off in (0, 64, 128))
+    src = [rnd(20 + n, (B, N, H, D), torch.bfloat16) for n in range(3)]
+    for t, s in zip((q, k, v), src):
+        t.copy_(s)
+    out = ops().window_attention(q, k, v, left=8, right=2, sinks=1)
+    assert torch.equal(out, ops().window_attention(*src, left=8, right=2, sinks=1))
+    lens = torch.tensor([40, 33], dtype=torch.int32, device="cuda")
+    assert torch.equal(ops().window_attention_step(q[:, -2:], k, v, lens, left=8, sinks=1),
+                       ops().window_attention_step(src[0][:, -2:].contiguous(), src[1], src[2], lens, left=8, sinks=1))
+
+
+# B, T, S, H, G, D, left, sinks, lengths
+STEP = [
+    (1, 1, 1, 1, 1, 64, None, 0, [1]),
+    (2, 1, 70, 4, 2, 64, 20, 3, [70, 5]),
+    (3, 1, 100, 8, 1, 128, None, 0, [0, 64, 100]),           # an empty sequence
+    (2, 3, 80, 6, 2, 40, 33, 40, [80, 2]),                    # rows in front of the first position
+    (1, 5, 600, 8, 1, 32, 500, 7, [599]),                     # 40 columns: two tiles of them
+    (1, 1, 5000, 4, 1, 64, None, 0, [4999]),                  # split over workgroups
+    (2, 2, 9000, 16, 2, 128, 8191, 40, [9000, 8500]),
+    (1, 1, 3000, 2, 2, 8, 100, 16, [2999]),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(STEP)))
+def test_window_attention_step(case, dtype):
+    B, T, S, H, G, D, left, sinks, lens = STEP[case]
+    q, k, v = rnd(31, (B, T, H, D), dtype), rnd(32, (B, S, G, D), dtype), rnd(33, (B, S, G, D), dtype)
+    for b, n in enumerate(lens):                              # what lies behind a sequence is not read
+        k[b, n:] = math.nan
+        v[b, n:] = math.inf
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out = ops().window_attention_step(q, k, v, lengths, left=left, sinks=sinks)
+    O.check(f"{dtype} {STEP[case]}", out, O.attention(q, k, v, left, 0, sinks, lens, step=True, dtype=dtype)["out"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_step_continues_a_causal_pass(dtype):
+    """The cache of a causal pass, then its last rows one at a time and together: the same numbers as the whole pass's, to rounding."""
+    B, N, H, G, D = 2, 140, 4, 2, 64
+    q, k, v = rnd(34, (B, N, H, D), dtype), rnd(35, (B, N, G, D), dtype), rnd(36, (B, N, G, D), dtype)
+    want = O.attention(q, k, v, 30, 0, 2, None, dtype=dtype)["out"]
+    whole = ops().window_attention(q, k, v, left=30, right=0, sinks=2)
+    O.check("whole", whole, want)
+    for n in (1, 2, 31, 140):
+        one = ops().window_attention_step(q[:, n - 1:n], k, v, torch.full((B,), n, device="cuda"), left=30, sinks=2)
+        O.check(f"row {n}", one, tuple(t[:, n - 1:n] for t in want))
+    four = ops().window_attention_step(q[:, -4:], k, v, torch.full((B,), N, device="cuda"), left=30, sinks=2)
+    O.check("four", four, tuple(t[:, -4:] for t in want))
+
+
+ROTARY = [
+    # B, N, H, G, D, axes, pairs, layout, positions, far
+    (2, 5, 2, 1, 64, 1, 32, "half", torch.int32, 100),
+    (1, 1, 8, 2, 64, 1, 32, "interleaved", torch.int64, 10 ** 9),
+    (3, 40, 4, 4, 64, 3, 10, "interleaved", torch.float32, 30),
+    (2, 17, 1, 2, 128, 2, 16, "half", torch.float32, 5),
+    (1, 300, 3, 1, 40, 1, 7, "half", torch.int64, 10 ** 6),       # pairs that do not fill a vector, channels that stay
+    (1, 33, 1, 1, 30, 3, 5, "interleaved", torch.int32, 50),
+    (1, 9, 2, 2, 7, 1, 3, "interleaved", torch.int32, 50),        # an odd head
+    (2, 2000, 2, 2, 16, 1, 8, "half", torch.int64, 10 ** 5),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(ROTARY)))
+def test_rotary_forward_and_gradients(case, dtype):
+    B, N, H, G, D, axes, P, layout, pt, far = ROTARY[case]
+    q, k = rnd(41, (B, N, H, D), dtype).requires_grad_(), rnd(42, (B, N, G, D), dtype).requires_grad_()
+    g = torch.Generator().manual_seed(43)
+    pos = (torch.rand((B, N) if axes == 1 else (B, N, axes), generator=g, dtype=torch.float64) * 2 * far - far).to(pt).cuda()
+    freqs, mag = ops().rotary_frequencies(P, scaling="parts", factor=4.0, original_length=64, device="cuda")
+    qr, kr = ops().rotary(q, k, pos, freqs, magnitude=mag, layout=layout)
+    gq, gk = rnd(44, q.shape, dtype), rnd(45, k.shape, dtype)
+    dq, dk = torch.autograd.grad((qr, kr), (q, k), (gq, gk))
+    for name, got, x, sign in (("q", qr, q, 1.0), ("k", kr, k, 1.0), ("dq", dq, gq, -1.0), ("dk", dk, gk, -1.0)):
+        O.check(f"{name} {dtype} {ROTARY[case]}", got, O.rotary(x, pos, freqs, mag, layout, sign, dtype))
+    alone = ops().rotary(q.detach(), None, pos, freqs, magnitude=mag, layout=layout)
+    assert torch.equal(alone, qr)
+    dq1, = torch.autograd.grad(ops().rotary(q, k, pos, freqs, magnitude=mag, layout=layout)[0], (q,), gq)
+    assert torch.equal(dq1, dq)
+
+
+def test_rotary_strides_and_broadcast_positions():
+    for dtype in TYPES:
+        packed = rnd(46, (2, 50, 3, 64), dtype)
+        q, k = packed[:, :, :2], packed[:, :, 2:]
+        freqs, mag = ops().rotary_frequencies(32, device="cuda")
+        pos = torch.arange(50, device="cuda")
+        want = ops().rotary(q.contiguous(), k.contiguous(), pos.expand(2, 50).contiguous(), freqs)
+        got = ops().rotary(q, k, pos, freqs)
+        assert mag == 1.0
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), (dtype, float((a.double() - b.double()).abs().max()))
+        cut = rnd(46, (2, 50, 3, 66), dtype)[..., 1:65]            # not aligned
+        # the element-wise form may round half values once (a mixed-precision fma) where the vector form rounds twice: both are held to
+        # the value's bound, not to each other
+        for y in ops().rotary(cut, cut, pos, freqs):
+            O.check("unaligned", y, O.rotary(cut, pos, freqs, 1.0, "half", 1.0, dtype))
+
+
+@pytest.mark.parametrize("scaling,factor", [(None, 1.0), ("linear", 4.0), ("base", 8.0), ("parts", 4.0)])
+def test_rotary_frequencies_turn_as_documented(scaling, factor):
+    P, base, length = 32, 10000.0, 4096.0
+    f, mag = ops().rotary_frequencies(P, base, scaling, factor, length)
+    plain = torch.tensor([base ** (-p / P) for p in range(P)], dtype=torch.float64)
+    ratio = plain / f
+    if scaling is None:
+        assert torch.allclose(ratio, torch.ones_like(ratio), rtol=1e-12)
+    elif scaling == "linear":
+        assert torch.allclose(ratio, torch.full_like(ratio, factor), rtol=1e-12)
+    elif scaling == "base":
+        assert abs(float(ratio[0]) - 1) < 1e-12 and abs(float(ratio[-1]) - factor) < 1e-9 and bool((ratio[1:] > ratio[:-1]).all())
+    else:
+        turns = length * plain / (2 * math.pi)
+        assert bool((ratio[turns >= 40] < 1 + 1e-12).all()) and bool((ratio[turns <= 0.75] > factor - 1e-9).all())
+        assert abs(mag - (0.1 * math.log(factor) + 1)) < 1e-15
+
+
+NORM = [(1, 1), (3, 7), (5, 64), (130, 72), (2, 129), (64, 192), (33, 256), (700, 200), (9, 512), (4, 1000), (3, 2048), (2, 4095), (2, 5000), (1, 16384)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["none", "same", "f32"])
+@pytest.mark.parametrize("rows,C", NORM)
+def test_rms_norm_forward_and_gradients(rows, C, kind, dtype):
+    x = rnd(51, (rows, C), dtype).requires_grad_()
+    wt = torch.float32 if (rows + C) % 2 else dtype
+    w = (1 + 0.2 * rnd(52, (C,), torch.float32)).to(wt).requires_grad_()
+    r = None if kind == "none" else rnd(53, (rows, C), dtype if kind == "same" else torch.float32).requires_grad_()
+    dy = rnd(54, (rows, C), dtype)
+    ds = None if r is None else rnd(55, (rows, C), r.dtype)
+    got = ops().rms_norm(x, w, 1e-5, residual=r)
+    want = O.rms(x, w, 1e-5, r, dy, ds)
+    if r is None:
+        O.check("y", got, want["y"])
+        dx, dw = torch.autograd.grad(got, (x, w), dy)
+    else:
+        O.check("y", got[0], want["y"])
+        assert torch.equal(got[1].detach().cpu().double(), want["stream"][0])
+        dx, dw, dr = torch.autograd.grad(got, (x, w, r), (dy, ds))
+        O.check("dr", dr, want["dr"])
+    O.check("dx", dx, want["dx"])
+    O.check("dw", dw, (want["dw"][0], want["dw"][1] + O.u(wt) * want["dw"][0].abs()))
+    with torch.no_grad():
+        again = ops().rms_norm(x, w, 1e-5, residual=r)
+    for a, b in zip((again,) if r is None else again, (got,) if r is None else got):
+        assert torch.equal(a, b)
+
+
+def test_rms_norm_partial_gradients_and_strides():
+    x, w, r = rnd(56, (4, 9, 128), torch.bfloat16).requires_grad_(), torch.ones(128, device="cuda", requires_grad=True), rnd(57, (4, 9, 128), torch.float32).requires_grad_()
+    y, s = ops().rms_norm(x, w, residual=r)
+    full = torch.autograd.grad((y, s), (x, w, r), (torch.ones_like(y), torch.zeros_like(s)), retain_graph=True)
+    only_y = torch.autograd.grad(y, (x, w, r), torch.ones_like(y), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(full, only_y))
+    gs = rnd(58, s.shape, torch.float32)
+    dx, dw, dr = torch.autograd.grad(s, (x, w, r), gs, allow_unused=True)
+    assert torch.equal(dr, gs) and torch.equal(dx, gs.bfloat16()) and (dw is None or not dw.any())
+    wide = rnd(59, (12, 300), torch.float16)
+    for cut in (wide[:, 3:203], wide[:, 8:208], wide[::2, :200], wide.t()[:12]):
+        w16 = torch.ones(cut.shape[1], dtype=torch.float16, device="cuda")
+        assert torch.equal(ops().rms_norm(cut, w16), ops().rms_norm(cut.contiguous(), w16))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,C,group", [(1, 8, None), (7, 64, 32), (5, 100, None), (40, 128, 128), (9, 256, 64), (3, 384, 128),
+                                          (6, 1024, 128), (2, 4096, 128), (3, 4096, None), (1, 16384, 64), (2, 2056, None)])
+def test_rms_norm_fp8(rows, C, group, dtype):
+    x, r = rnd(61, (rows, C), dtype, 3.0), rnd(62, (rows, C), dtype)
+    w = 1 + 0.2 * rnd(63, (C,), torch.float32)
+    if rows > 1:
+        x[1], r[1] = 0, 0                                     # a row of zeros
+    q, scale, s = ops().rms_norm_fp8(x, w, 1e-6, residual=r, group=group)
+    want = O.rms(x, w, 1e-6, r)
+    assert q.dtype == torch.float8_e4m3fn and torch.equal(s.cpu().double(), want["stream"][0])
+    y = want["y"][0].view(rows, -1, group or C)
+    sc = y.abs().amax(-1).clamp_min(1e-12) / 448
+    O.check("scale", scale.view(rows, -1), (sc, 56 * O.U32 * sc))
+    got = q.float().cpu().double().view_as(y) * scale.cpu().double().view(rows, -1, 1)
+    # half a step of e4m3: 2^-4 of the value, 2^-10 scales where it is subnormal
+    assert bool(((got - y).abs() <= (2.0 ** -4 + 1e-5) * y.abs() + 2.0 ** -10 * 1.0001 * sc[..., None]).all())
+    if rows > 1:
+        assert not q[1].float().any() and bool((scale[1] > 0).all())
+
+
+def test_rms_norm_fp8_keeps_nan():
+    x = torch.ones((2, 64), device="cuda")
+    x[0, 5] = math.nan
+    q, scale = ops().rms_norm_fp8(x, torch.ones(64, device="cuda"), group=32)
+    assert bool(scale[0].isnan().all()) and bool(q[0].float().isnan().all()) and bool(q[1].float().isfinite().all())
+
+
+def _layer(o, h, branch, w, wqkv, pos, freqs, H, G, D, lengths):
+    """A pre-norm attention layer as it would be used: residual norm, one projection, rotary positions, window attention."""
+    y, h = o.rms_norm(branch, w, residual=h)
+    B, N, _ = y.shape
+    qkv = (y @ wqkv).view(B, N, H + 2 * G, D)
+    q, k = o.rotary(qkv[:, :, :H], qkv[:, :, H:H + G], pos, freqs)
+    return h, o.window_attention(q, k, qkv[:, :, H + G:], left=24, right=24, sinks=2, lengths=lengths).reshape(B, N, H * D)
+
+
+def test_a_layer_of_them_together_and_replayed():
+    """The operators in a row: against the float64 forms in fp32, and a training step captured into a graph and replayed with new
+    inputs between eager work, equal to the eager step."""
+    o = ops()
+    B, N, H, G, D = 2, 75, 4, 2, 32
+    C = H * D
+    freqs, _ = o.rotary_frequencies(D // 2, device="cuda")
+    pos = torch.arange(N, device="cuda")
+    lengths = torch.tensor([75, 60], dtype=torch.int32, device="cuda")
+    new = lambda n: (rnd(70 + n, (B, N, C), torch.float32), rnd(80 + n, (B, N, C), torch.float32))  # noqa: E731
+    w, wqkv = (1 + 0.1 * rnd(71, (C,), torch.float32)).requires_grad_(), (rnd(72, (C, (H + 2 * G) * D), torch.float32) / C ** 0.5).requires_grad_()
+    h, x = (t.clone() for t in new(0))
+
+    def step():
+        s, y = _layer(o, h, x, w, wqkv, pos, freqs, H, G, D, lengths)
+        return (s, y) + torch.autograd.grad((s + y).square().sum(), (w, wqkv))
+
+    # (no eager graph over w and wqkv may live while a backward through them is captured: torch would make its streams part of the
+    # capture, which ends the process)
+    with torch.no_grad():
+        s, y = _layer(o, h, x, w, wqkv, pos, freqs, H, G, D, lengths)
+    rs = O.rms(x, w, 1e-6, h)
+    qkv = (rs["y"][0] @ wqkv.detach().cpu().double()).view(B, N, H + 2 * G, D)
+    q, k = (O.rotary(t, pos, freqs, 1.0, "half")[0] for t in (qkv[:, :, :H], qkv[:, :, H:H + G]))
+    want = O.attention(q, k, qkv[:, :, H + G:], 24, 24, 2, [75, 60])["out"][0].reshape(B, N, C)
+    # the projection's fp32 product of C = 128 terms is off by C u32 relative, about 1e-5 of values of a few units
+    assert float((y.detach().cpu().double() - want).abs().max()) < 2e-4
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for n in range(4):
+        a, b = new(n)
+        h.copy_(a), x.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, eager in zip(held, step()):
+            assert torch.equal(got, eager)
+
+
+def test_other_streams():
+    q, k, v = (rnd(90 + n, (1, 500, 2, 64), torch.bfloat16) for n in range(3))
+    lens = torch.tensor([500], dtype=torch.int32, device="cuda")
+    want = ops().window_attention(q, k, v, left=60, right=60), ops().window_attention_step(q[:, -1:], k, v, lens)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for st in streams:
+        with torch.cuda.stream(st):
+            got.append((ops().window_attention(q, k, v, left=60, right=60), ops().window_attention_step(q[:, -1:], k, v, lens)))
+    torch.cuda.synchronize()
+    for pair in got:
+        assert all(torch.equal(a, b) for a, b in zip(pair, want))
