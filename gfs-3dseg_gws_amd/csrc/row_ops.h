@@ -379,20 +379,22 @@ __global__ void __launch_bounds__(256) rms_bwd_kernel(const RnArgs g)
         for (int c = threadIdx.x; c < g.C; c += 256) o[c] = rn_dw[c];
     }
 }
-// dw[c] = sum over the parts, in order within each of 8 slices, then over the slices
+// dw[c] = sum over the parts, in order within each of 32 slices, then over the slices
 template <class W>
-__global__ void __launch_bounds__(256) rms_dw_kernel(const float *__restrict__ part, int nparts, int C, W *__restrict__ dw)
+__global__ void __launch_bounds__(1024) rms_dw_kernel(const float *__restrict__ part, int nparts, int C, W *__restrict__ dw)
 {
-    __shared__ float sh[8][32];
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), sl = threadIdx.x >> 5;
+    __shared__ float sh[32][33];
+    const int tc = threadIdx.x & 31, c = blockIdx.x * 32 + tc, sl = threadIdx.x >> 5;
     float s = 0.f;
-    if (c < C)
-        for (int p = sl; p < nparts; p += 8) s += part[(size_t)p * C + c];
-    sh[sl][threadIdx.x & 31] = s;
+    if (c < C) {
+#pragma unroll 8
+        for (int p = sl; p < nparts; p += 32) s += part[(size_t)p * C + c];
+    }
+    sh[sl][tc] = s;
     __syncthreads();
     if (sl == 0 && c < C) {
 #pragma unroll
-        for (int k = 1; k < 8; ++k) s += sh[k][threadIdx.x];
+        for (int k = 1; k < 32; ++k) s += sh[k][tc];
         dw[c] = (W)s;
     }
 }
@@ -571,9 +573,9 @@ extern "C" int gfs3d_rms_norm_backward(const gfs3d_rms_norm_args *a, void *strea
     else rc = rn_backward<_Float16>(g, parts, st);
     if (rc || !a->dweight) return rc;
     const dim3 grid((a->C + 31) / 32);
-    if (g.wf32) hipLaunchKernelGGL((rms_dw_kernel<float>), grid, dim3(256), 0, st, g.part, parts, a->C, (float *)a->dweight);
-    else if (a->type == GFS3D_COMPUTE_BF16) hipLaunchKernelGGL((rms_dw_kernel<__bf16>), grid, dim3(256), 0, st, g.part, parts, a->C, (__bf16 *)a->dweight);
-    else hipLaunchKernelGGL((rms_dw_kernel<_Float16>), grid, dim3(256), 0, st, g.part, parts, a->C, (_Float16 *)a->dweight);
+    if (g.wf32) hipLaunchKernelGGL((rms_dw_kernel<float>), grid, dim3(1024), 0, st, g.part, parts, a->C, (float *)a->dweight);
+    else if (a->type == GFS3D_COMPUTE_BF16) hipLaunchKernelGGL((rms_dw_kernel<__bf16>), grid, dim3(1024), 0, st, g.part, parts, a->C, (__bf16 *)a->dweight);
+    else hipLaunchKernelGGL((rms_dw_kernel<_Float16>), grid, dim3(1024), 0, st, g.part, parts, a->C, (_Float16 *)a->dweight);
     GFS3D_LAUNCH_CHECK("rms_dw_kernel");
     return GFS3D_OK;
 }

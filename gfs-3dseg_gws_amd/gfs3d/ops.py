@@ -1457,19 +1457,16 @@ class KMeansDelta:
 _TYPE_IDS = {torch.float32: _lib.COMPUTE_F32, torch.bfloat16: _lib.COMPUTE_BF16, torch.float16: _lib.COMPUTE_F16}
 
 
-def _need_typed(who: str, **tensors) -> torch.device:
-    """All given tensors on one GPU and of one supported type."""
-    device = dtype = None
-    for name, t in tensors.items():
+def _need_typed(who: str, first: torch.Tensor, *rest: torch.Tensor) -> int:
+    """All given tensors on one GPU and of one supported type; returns the GPU's index."""
+    for t in (first,) + rest:
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
-            raise RuntimeError(f"gfs3d.{who}: `{name}` must be a HIP (cuda) tensor - the hot path has no CPU fallback")
+            raise RuntimeError(f"gfs3d.{who}: every input must be a HIP (cuda) tensor - the hot path has no CPU fallback")
         if t.dtype not in _TYPE_IDS:
-            raise RuntimeError(f"gfs3d.{who}: `{name}` must be float32, bfloat16 or float16, got {t.dtype}")
-        if device is None:
-            device, dtype = t.device, t.dtype
-        elif t.device != device or t.dtype != dtype:
-            raise RuntimeError(f"gfs3d.{who}: `{name}` is {t.dtype} on {t.device}, the first tensor {dtype} on {device}")
-    return device
+            raise RuntimeError(f"gfs3d.{who}: inputs must be float32, bfloat16 or float16, got {t.dtype}")
+        if t.dtype is not first.dtype or t.get_device() != first.get_device():
+            raise RuntimeError(f"gfs3d.{who}: inputs differ: {t.dtype} on {t.device} beside {first.dtype} on {first.device}")
+    return first.get_device()
 
 
 def _no_grad_form(who: str, *tensors) -> None:
@@ -1477,14 +1474,15 @@ def _no_grad_form(who: str, *tensors) -> None:
         raise RuntimeError(f"gfs3d.{who} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
-def _launch(fn: str, device: torch.device, args) -> None:
+def _launch(fn: str, device: int, args) -> None:
     call = getattr(_lib.lib(), fn)
-    if device.index == torch.cuda.current_device():
-        rc = call(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
+    if device == torch._C._cuda_getDevice():
+        rc = call(args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            rc = call(ctypes.byref(args), torch._C._cuda_getCurrentRawStream(device.index))
-    _lib.check(rc, fn)
+            rc = call(args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != 0:
+        _lib.check(rc, fn)
 
 
 def _heads4(t: torch.Tensor) -> torch.Tensor:
@@ -1497,47 +1495,43 @@ def _heads4(t: torch.Tensor) -> torch.Tensor:
 
 
 def _window_args(who, q, k, v, left, right, sinks, scale, lengths):
-    device = _need_typed(who, q=q, k=k, v=v)
+    device = _need_typed(who, q, k, v)
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or k.shape[0] != q.shape[0] or k.shape[3] != q.shape[3]:
         raise RuntimeError(f"gfs3d.{who}: q must be (B, N, H, D), k and v (B, S, G, D), got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     B, N, H, D = q.shape
-    S, G = k.shape[1], k.shape[2]
+    _, S, G, _ = k.shape
     if G < 1 or H < 1 or H % G:
         raise RuntimeError(f"gfs3d.{who}: {H} heads do not divide over {G} key heads")
     if D < 8 or D > 128 or D % 8:
         raise NotImplementedError(f"gfs3d.{who}: head sizes are multiples of 8 up to 128, got {D}")
     if (left is not None and left < 0) or (right is not None and right < 0) or sinks < 0:
         raise RuntimeError(f"gfs3d.{who}: left, right and sinks must not be negative")
-    scale = 1.0 / D ** 0.5 if scale is None else float(scale)
+    scale = D ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 3e38:
         raise RuntimeError(f"gfs3d.{who}: scale must be positive and finite, got {scale}")
     if lengths is not None:
-        if not isinstance(lengths, torch.Tensor) or lengths.device != device or lengths.dtype not in (torch.int32, torch.int64) \
+        if not isinstance(lengths, torch.Tensor) or lengths.get_device() != device or lengths.dtype not in (torch.int32, torch.int64) \
                 or tuple(lengths.shape) != (B,):
-            raise RuntimeError(f"gfs3d.{who}: lengths must be an int32 or int64 tensor of shape ({B},) on {device}")
-        if lengths.dtype == torch.int64:
+            raise RuntimeError(f"gfs3d.{who}: lengths must be an int32 or int64 tensor of shape ({B},) on {q.device}")
+        if lengths.dtype is torch.int64:
             lengths = lengths.clamp(0, S).to(torch.int32)
         lengths = lengths.contiguous()
-    a = _lib.WindowAttnArgs()
-    a.B, a.N, a.S, a.H, a.G, a.D, a.type = B, N, S, H, G, D, _TYPE_IDS[q.dtype]
-    a.left = S if left is None else min(int(left), S)
-    a.right = S if right is None else min(int(right), S)
-    a.sinks, a.scale = min(int(sinks), S), scale
-    a.lengths = lengths.data_ptr() if lengths is not None else None
-    return a, lengths
+    a = _lib.WindowAttnArgs(B, N, S, H, G, D, _TYPE_IDS[q.dtype], S if left is None else min(int(left), S), S if right is None else min(int(right), S),
+                            min(int(sinks), S), scale)
+    if lengths is not None:
+        a.lengths = lengths.data_ptr()
+    return a, lengths, device
 
 
 def _window_inputs(a, q, k, v):
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        setattr(a, name, t.data_ptr())
-        s = t.stride()
-        setattr(a, name + "_stride", (ctypes.c_longlong * 3)(s[0], s[1], s[2]))
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_stride, a.k_stride, a.v_stride = q.stride()[:3], k.stride()[:3], v.stride()[:3]
 
 
 class WindowAttentionFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, left, right, sinks, scale, lengths):
-        a, lengths = _window_args("window_attention", q, k, v, left, right, sinks, scale, lengths)
+        a, lengths, device = _window_args("window_attention", q, k, v, left, right, sinks, scale, lengths)
         if a.S != a.N:
             raise RuntimeError(f"gfs3d.window_attention: q has {a.N} rows, k and v {a.S} (the last rows of a cache: window_attention_step)")
         q, k, v = _heads4(q), _heads4(k), _heads4(v)
@@ -1547,7 +1541,7 @@ class WindowAttentionFunction(torch.autograd.Function):
         if out.numel():
             _window_inputs(a, q, k, v)
             a.out, a.lse = out.data_ptr(), lse.data_ptr() if grad else None
-            _launch("gfs3d_window_attn_forward", q.device, a)
+            _launch("gfs3d_window_attn_forward", device, a)
         if grad:
             ctx.save_for_backward(q, k, v, out, lse, lengths)
             ctx.cfg = (left, right, sinks, scale)
@@ -1557,18 +1551,17 @@ class WindowAttentionFunction(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         q, k, v, out, lse, lengths = ctx.saved_tensors
-        a, _ = _window_args("window_attention", q, k, v, *ctx.cfg, lengths)
+        a, _, device = _window_args("window_attention", q, k, v, *ctx.cfg, lengths)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         if out.numel():
             dout = _heads4(dout)
             _window_inputs(a, q, k, v)
             a.out, a.lse, a.dout, a.dq, a.dk, a.dv = (t.data_ptr() for t in (out, lse, dout, dq, dk, dv))
-            s = dout.stride()
-            a.dout_stride = (ctypes.c_longlong * 3)(s[0], s[1], s[2])
+            a.dout_stride = dout.stride()[:3]
             nbytes = _lib.lib().gfs3d_window_attn_workspace_bytes(a.B, a.N, a.S, a.H, a.G, a.D, a.left, a.sinks, 0)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # from torch's allocator: a captured graph keeps its own
             a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-            _launch("gfs3d_window_attn_backward", q.device, a)
+            _launch("gfs3d_window_attn_backward", device, a)
         return dq, dk, dv, None, None, None, None, None
 
 
@@ -1590,7 +1583,7 @@ def window_attention_step(q, k, v, lengths, left: Optional[int] = None, sinks: i
     _no_grad_form("window_attention_step", q, k, v)
     if lengths is None:
         raise RuntimeError("gfs3d.window_attention_step: lengths (B,) is needed")
-    a, lengths = _window_args("window_attention_step", q, k, v, left, 0, sinks, scale, lengths)
+    a, lengths, device = _window_args("window_attention_step", q, k, v, left, 0, sinks, scale, lengths)
     out = torch.empty((a.B, a.N, a.H, a.D), dtype=q.dtype, device=q.device)
     if out.numel() == 0 or a.S == 0:
         return out.zero_()
@@ -1599,8 +1592,9 @@ def window_attention_step(q, k, v, lengths, left: Optional[int] = None, sinks: i
     a.out = out.data_ptr()
     nbytes = _lib.lib().gfs3d_window_attn_workspace_bytes(a.B, a.N, a.S, a.H, a.G, a.D, a.left, a.sinks, 1)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    a.workspace, a.workspace_bytes = (ws.data_ptr(), nbytes) if nbytes else (None, 0)
-    _launch("gfs3d_window_attn_step", q.device, a)
+    if nbytes:
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _launch("gfs3d_window_attn_step", device, a)
     return out
 
 
@@ -1637,31 +1631,23 @@ def rotary_frequencies(pairs: int, base: float = 10000.0, scaling: Optional[str]
 
 
 def _rotary_launch(q, k, positions, freqs, magnitude, interleaved, inverse):
-    a = _lib.RotaryArgs()
     B, N, H, D = q.shape
-    a.B, a.N, a.D, a.type = B, N, D, _TYPE_IDS[q.dtype]
-    outs = []
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            outs.append(None)
-            continue
-        if t.stride(3) != 1:
-            t = t.contiguous()
-        o = torch.empty(t.shape, dtype=t.dtype, device=t.device)
-        setattr(a, name, t.data_ptr())
-        setattr(a, name + "_out", o.data_ptr())
-        setattr(a, name + "_heads", t.shape[2])
-        s = t.stride()
-        setattr(a, name + "_stride", (ctypes.c_longlong * 3)(s[0], s[1], s[2]))
-        s = o.stride()
-        setattr(a, name + "_out_stride", (ctypes.c_longlong * 3)(s[0], s[1], s[2]))
-        outs.append((o, t))                                   # t: kept until the launch
-    a.positions, a.position_type, a.axes = positions.data_ptr(), _POSITION_IDS[positions.dtype], positions.shape[2]
-    a.pairs, a.interleaved, a.inverse = freqs.numel(), interleaved, inverse
-    a.freqs, a.magnitude = freqs.data_ptr(), magnitude
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    qo = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
+    kp, kop, ks, kos, G, ko = None, None, (0, 0, 0), (0, 0, 0), 0, None
+    if k is not None:
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        G = k.shape[2]
+        ko = torch.empty((B, N, G, D), dtype=k.dtype, device=k.device)
+        kp, kop, ks, kos = k.data_ptr(), ko.data_ptr(), k.stride()[:3], (N * G * D, G * D, D)
     if B and N:
-        _launch("gfs3d_rotary", q.device, a)
-    return tuple(o[0] if o is not None else None for o in outs)
+        _launch("gfs3d_rotary", q.get_device(), _lib.RotaryArgs(
+            B, N, D, _TYPE_IDS[q.dtype], H, G, q.data_ptr(), kp, qo.data_ptr(), kop, q.stride()[:3], ks, (N * H * D, H * D, D), kos,
+            positions.data_ptr(), _POSITION_IDS[positions.dtype], positions.shape[2], freqs.shape[0], interleaved, inverse,
+            freqs.data_ptr(), magnitude))
+    return qo, ko
 
 
 class RotaryFunction(torch.autograd.Function):
@@ -1692,23 +1678,23 @@ def rotary(q, k, positions, freqs, magnitude: float = 1.0, layout: str = "half")
     copied.  layout "half": pair p is the section's channels (p, P + p); "interleaved": (2 p, 2 p + 1).  positions (N,), (B, N) or
     (B, N, axes) with 1 to 3 axes (a point's coordinates, say), int32, int64 or float32; freqs (P,) float64 on the device
     (`rotary_frequencies`); angles are formed in float64.  Differentiable in q and k.  Returns (q', k'), or q' alone without k."""
-    device = _need_typed("rotary", q=q, **({"k": k} if k is not None else {}))
+    device = _need_typed("rotary", q) if k is None else _need_typed("rotary", q, k)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise RuntimeError("gfs3d.rotary: q must be (B, N, H, D) and k (B, N, G, D)")
     if layout not in ("half", "interleaved"):
         raise ValueError(f"gfs3d.rotary: layout must be \"half\" or \"interleaved\", got {layout!r}")
     B, N, H, D = q.shape
-    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_IDS or positions.device != device:
-        raise RuntimeError(f"gfs3d.rotary: positions must be an int32, int64 or float32 tensor on {device}")
+    if not isinstance(positions, torch.Tensor) or positions.dtype not in _POSITION_IDS or positions.get_device() != device:
+        raise RuntimeError(f"gfs3d.rotary: positions must be an int32, int64 or float32 tensor on {q.device}")
     if positions.dim() == 1:
         positions = positions.expand(B, positions.shape[0])
     if positions.dim() == 2:
         positions = positions[:, :, None]
     if positions.dim() != 3 or tuple(positions.shape[:2]) != (B, N) or not 1 <= positions.shape[2] <= 3:
         raise RuntimeError(f"gfs3d.rotary: positions must be ({N},), ({B}, {N}) or ({B}, {N}, 1..3), got {tuple(positions.shape)}")
-    if not isinstance(freqs, torch.Tensor) or freqs.dtype != torch.float64 or freqs.device != device or freqs.dim() != 1:
-        raise RuntimeError(f"gfs3d.rotary: freqs must be a 1-d float64 tensor on {device}")
-    P = freqs.numel()
+    if not isinstance(freqs, torch.Tensor) or freqs.dtype is not torch.float64 or freqs.get_device() != device or freqs.dim() != 1:
+        raise RuntimeError(f"gfs3d.rotary: freqs must be a 1-d float64 tensor on {q.device}")
+    P = freqs.shape[0]
     if P < 1 or 2 * P * positions.shape[2] > D or P * positions.shape[2] > 1024 or H < 1 or (k is not None and k.shape[2] < 1):
         raise RuntimeError(f"gfs3d.rotary: {positions.shape[2]} axes of {P} pairs do not fit heads of {D} channels")
     positions, freqs = positions.contiguous(), freqs.contiguous()
@@ -1725,48 +1711,40 @@ def _rows2(t: torch.Tensor) -> torch.Tensor:
     C = t.shape[-1]
     if t.stride(-1) != 1 and C > 1:
         t = t.contiguous()
-    return t.reshape(-1, C)
-
-
-def _rms_args(who, x, weight, eps, residual):
-    device = _need_typed(who, x=x)
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError(f"gfs3d.{who}: x must be (.., C)")
-    C = x.shape[-1]
-    if C > 16384:
-        raise NotImplementedError(f"gfs3d.{who}: rows of up to 16384 channels, got {C}")
-    if not isinstance(weight, torch.Tensor) or weight.device != device or weight.dtype not in (torch.float32, x.dtype) or tuple(weight.shape) != (C,):
-        raise RuntimeError(f"gfs3d.{who}: weight must be a ({C},) tensor of float32 or {x.dtype} on {device}")
-    if residual is not None and (not isinstance(residual, torch.Tensor) or residual.device != device or residual.shape != x.shape
-                                 or residual.dtype not in (torch.float32, x.dtype)):
-        raise RuntimeError(f"gfs3d.{who}: residual must have x's shape {tuple(x.shape)}, in float32 or {x.dtype}, on {device}")
-    if not 0.0 <= eps < 3e38:
-        raise RuntimeError(f"gfs3d.{who}: eps must not be negative, got {eps}")
-    a = _lib.RmsNormArgs()
-    a.rows, a.C, a.type = x.numel() // C, C, _TYPE_IDS[x.dtype]
-    a.residual_f32 = int(residual is not None and residual.dtype == torch.float32)
-    a.weight_f32 = int(weight.dtype == torch.float32)
-    a.eps, a.weight = float(eps), weight.data_ptr()
-    return a
+    return t if t.dim() == 2 else t.reshape(-1, C)
 
 
 def _rms_forward(who, x, weight, eps, residual, want_rstd=False, fp8=False, group=0):
-    """(y, scale or None, stream or None, rstd or None, the (rows, C) stream or x that the backward reads)."""
-    weight = weight.contiguous()
-    a = _rms_args(who, x, weight, eps, residual)
-    x2 = _rows2(x)
-    y = torch.empty(x.shape, dtype=torch.float8_e4m3fn if fp8 else x.dtype, device=x.device)
-    stream = torch.empty(x.shape, dtype=residual.dtype, device=x.device) if residual is not None else None
-    rstd = torch.empty(a.rows, dtype=torch.float32, device=x.device) if want_rstd else None
-    scale = torch.empty(x.shape[:-1] + ((a.C // group,) if group else ()), dtype=torch.float32, device=x.device) if fp8 else None
-    if a.rows:
-        a.x, a.x_stride, a.y = x2.data_ptr(), x2.stride(0), y.data_ptr()
-        if residual is not None:
-            r2 = _rows2(residual)
-            a.residual, a.r_stride, a.stream_out = r2.data_ptr(), r2.stride(0), stream.data_ptr()
-        a.rstd = rstd.data_ptr() if want_rstd else None
-        a.fp8, a.group, a.scale = int(fp8), group, scale.data_ptr() if fp8 else None
-        _launch("gfs3d_rms_norm_forward", x.device, a)
+    """(y, scale or None, stream or None, rstd or None, the (rows, C) view of x that the backward reads)."""
+    device = _need_typed(who, x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise RuntimeError(f"gfs3d.{who}: x must be (.., C)")
+    shape, dtype, C = x.shape, x.dtype, x.shape[-1]
+    if C > 16384:
+        raise NotImplementedError(f"gfs3d.{who}: rows of up to 16384 channels, got {C}")
+    if not isinstance(weight, torch.Tensor) or weight.get_device() != device or (weight.dtype is not torch.float32 and weight.dtype is not dtype) \
+            or tuple(weight.shape) != (C,):
+        raise RuntimeError(f"gfs3d.{who}: weight must be a ({C},) tensor of float32 or {dtype} on {x.device}")
+    if residual is not None and (not isinstance(residual, torch.Tensor) or residual.get_device() != device or residual.shape != shape
+                                 or (residual.dtype is not torch.float32 and residual.dtype is not dtype)):
+        raise RuntimeError(f"gfs3d.{who}: residual must have x's shape {tuple(shape)}, in float32 or {dtype}, on {x.device}")
+    if not 0.0 <= eps < 3e38:
+        raise RuntimeError(f"gfs3d.{who}: eps must not be negative, got {eps}")
+    weight, x2, dev = weight.contiguous(), _rows2(x), x.device
+    rows = x2.shape[0]
+    y = torch.empty(shape, dtype=torch.float8_e4m3fn if fp8 else dtype, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if want_rstd else None
+    scale = torch.empty(shape[:-1] + ((C // group,) if group else ()), dtype=torch.float32, device=dev) if fp8 else None
+    stream = r2 = None
+    if residual is not None:
+        r2 = _rows2(residual)
+        stream = torch.empty(shape, dtype=residual.dtype, device=dev)
+    if rows:
+        _launch("gfs3d_rms_norm_forward", device, _lib.RmsNormArgs(
+            rows, C, _TYPE_IDS[dtype], 1 if r2 is not None and r2.dtype is torch.float32 else 0, 1 if weight.dtype is torch.float32 else 0,
+            1 if fp8 else 0, group, eps, x2.data_ptr(), None if r2 is None else r2.data_ptr(), weight.data_ptr(), x2.stride(0),
+            0 if r2 is None else r2.stride(0), None if stream is None else stream.data_ptr(), y.data_ptr(),
+            None if scale is None else scale.data_ptr(), None if rstd is None else rstd.data_ptr()))
     return y, scale, stream, rstd, x2
 
 
@@ -1811,7 +1789,7 @@ class RmsNormFunction(torch.autograd.Function):
                 nbytes = _lib.lib().gfs3d_rms_norm_workspace_bytes(a.rows, a.C)
                 ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
                 a.dweight, a.workspace, a.workspace_bytes = dw.data_ptr(), ws.data_ptr(), nbytes
-            _launch("gfs3d_rms_norm_backward", s.device, a)
+            _launch("gfs3d_rms_norm_backward", s.get_device(), a)
         elif need_w:
             dw.zero_()
         return dx if need_x else None, dw, (dr if wide else dx) if need_r else None, None
