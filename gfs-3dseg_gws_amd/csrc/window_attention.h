@@ -116,19 +116,45 @@ __device__ __forceinline__ void wa_colfrags(const T *row, bool ok, int D, int h,
     }
 }
 
-// R rows of a (rows, D) matrix staged by NT threads: thread t takes the 8-channel chunks t, t + NT, ..
+// The per-wave operands are loaded before a loop whose own loads are still in flight when they are used: having them arrive here
+// keeps the compiler from waiting, in every turn, for everything that is in flight
+template <int A, int B> __device__ __forceinline__ void wa_settle(uint4 (&f)[A][B])
+{
+#pragma unroll
+    for (int a = 0; a < A; ++a)
+#pragma unroll
+        for (int b = 0; b < B; ++b) asm volatile("" : "+v"(f[a][b].x), "+v"(f[a][b].y), "+v"(f[a][b].z), "+v"(f[a][b].w));
+}
+
+// R rows of a (rows, D) matrix staged by NT threads: thread t takes the 8-channel chunks t, t + NT, ..  A chunk's place relative to the
+// tile's first row is fixed: 32-bit offsets from a base that is the same for all threads (scalar), no address arithmetic per tile
 template <class T, int DP, int R, int NT> struct WaStage {
     static constexpr int CPR = DP / 8, NCH = (R * CPR + NT - 1) / NT;
     static constexpr bool RAGGED = R * CPR % NT != 0;
     WaRaw<T> r[NCH];
-    // rows [row0, row0 + R) at `base` (row row0), rows >= end and channels >= D read as zeros
-    __device__ __forceinline__ void load(const T *base, long long stride, int row0, int end, int D, int t)
+    unsigned off[NCH];
+    __device__ __forceinline__ void init(long long stride, int t)
     {
 #pragma unroll
         for (int n = 0; n < NCH; ++n) {
-            const int c = t + n * NT, row = c / CPR, ch = 8 * (c % CPR);
-            r[n] = wa_zero<T>();
-            if ((!RAGGED || c < R * CPR) && row0 + row < end && ch < D) r[n] = wa_load8<T>(base + (long long)row * stride + ch);
+            const int c = t + n * NT;
+            off[n] = RAGGED && c >= R * CPR ? 0u : (unsigned)(c / CPR) * (unsigned)(stride * sizeof(T)) + (unsigned)(c % CPR) * (unsigned)(8 * sizeof(T));
+        }
+    }
+    // the R rows from `base` on; of them `left` are there, rows behind and channels >= D read as zeros
+    __device__ __forceinline__ void load(const T *base, int left, int D, int t)
+    {
+        const char *p = reinterpret_cast<const char *>(base);
+        if (left >= R && D == DP) {
+#pragma unroll
+            for (int n = 0; n < NCH; ++n) r[n] = *reinterpret_cast<const WaRaw<T> *>(p + off[n]);
+        } else {
+#pragma unroll
+            for (int n = 0; n < NCH; ++n) {
+                const int c = t + n * NT;
+                r[n] = wa_zero<T>();
+                if ((!RAGGED || c < R * CPR) && c / CPR < left && 8 * (c % CPR) < D) r[n] = *reinterpret_cast<const WaRaw<T> *>(p + off[n]);
+            }
         }
     }
     template <int PREC> __device__ __forceinline__ void put(unsigned char *img, int t) const
@@ -166,9 +192,88 @@ __device__ __forceinline__ unsigned wa_order(unsigned id, unsigned total)
 }
 constexpr float WA_LAZY = 8.f;        // the running maximum may lag the true one by 2^8: p, its sum and its products stay in range in fp32 and half
 
+// Hides what the lane does not see among the 32 rows from j0 on in its C/D registers: x[r] = fill unless row j = j0 + at_drow(r, h)
+// has lo <= j <= hi, or j < far (FAR: the sinks the lane sees).  One unsigned comparison per element for the window (hi >= lo - 1).
+template <bool FAR, class X> __device__ __forceinline__ void wa_mask(int j0, int h, int lo, int hi, int far, float fill, X &x)
+{
+    asm volatile("");                                 // keeps the branch around it: as selects the mask cost every tile its arithmetic
+    const int base = j0 + 4 * h - lo, fb = far - j0 - 4 * h;
+    const unsigned n = (unsigned)(hi - lo + 1);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        float y = (unsigned)(base + at_drow(r, 0)) < n ? x[r] : fill;
+        if (FAR) y = at_drow(r, 0) < fb ? x[r] : y;
+        x[r] = y;
+    }
+}
+
 // ------------------------------------------------------------------ forward
+// NS 32-key subtiles of the staged tile, from Kc / Vc on (keys j0 ..): scores, running softmax, products.  `whole`: every key is seen
+template <class T, int DP, int NS>
+__device__ __forceinline__ void wa_fwd_tile(const unsigned char *Kc, const unsigned char *Vc, int j0, int lane, float c, float thr, bool whole,
+                                            int lo, int hi, int far, const uint4 (&qp)[DP / 16][Mx<WaT<T>::PF>::NP], float &m, float &mc,
+                                            float &l, f32x16 (&O)[DP / 32])
+{
+    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, KT = WaT<T>::KT, ROWB = WaImg<DP>::ROWB, ND = DP / 32;
+    const int j = lane & 31, h = lane >> 5;
+    f32x16 acc[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[s][r] = 0.f;
+#pragma unroll
+        for (int kb = 0; kb < DP / 16; ++kb) {
+            uint4 ak[NP];
+            wa_rowfrag<PREC, DP, KT>(Kc, 32 * s + j, h, kb, ak);
+            mm_mac<PREC>(ak, qp[kb], acc[s]);
+        }
+    }
+    if (!whole) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            if (j0 + 32 * s >= far) wa_mask<false>(j0 + 32 * s, h, lo, hi, 0, -__builtin_inff(), acc[s]);
+            else wa_mask<true>(j0 + 32 * s, h, lo, hi, min(far, hi + 1), -__builtin_inff(), acc[s]);
+        }
+    }
+    float tmax = acc[0][0];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, acc[s][r]);
+    tmax = wa_max32(tmax);
+    if (__ballot(tmax > m + thr) != 0ull) {
+        const float m_new = fmaxf(m, tmax), mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c;
+        const float sc = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mc - mc_new);
+        m = m_new;
+        mc = mc_new;
+        l *= sc;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) O[d][r] *= sc;
+    }
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        float pd[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            pd[r] = __builtin_amdgcn_exp2f(fmaf(acc[s][r], c, -mc));
+            l += pd[r];
+        }
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+            uint4 pp[NP], av[NP];
+            at_regfrag<PREC>(pd, ks, pp);
+#pragma unroll
+            for (int d = 0; d < ND; ++d) {
+                wa_trfrag<PREC, DP, KT>(Vc + 32 * s * ROWB, lane, d, ks, av);
+                mm_mac<PREC>(av, pp, O[d]);
+            }
+        }
+    }
+}
 template <class T, int DP>
-__global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_fwd_kernel(const WaArgs g, T *__restrict__ out)
+__global__ void __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4 ? 3 : 4) wa_fwd_kernel(const WaArgs g, T *__restrict__ out)
 {
     constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, KT = WaT<T>::KT, SUB = KT / 32, IMG = NP * KT * WaImg<DP>::ROWB;
     constexpr int ROWB = WaImg<DP>::ROWB, ND = DP / 32;
@@ -195,84 +300,37 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_f
     const int tlo = max(0, qa - g.left) / KT, thi = min(len - 1, qb + g.right) / KT;
     const int nsink = min((min(g.sinks, len) + KT - 1) / KT, tlo);
     const int nt = qa < len ? nsink + thi - tlo + 1 : 0;
-    const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right);
+    const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right), far = min(g.sinks, len);
+    const int hi = min(len - 1, qi + g.right), lo = min(qi - g.left, hi + 1);
     const float thr = WA_LAZY / g.c;
     WaStage<T, DP, KT, 256> sk, sv;
+    sk.init(g.ks.r, t);
+    sv.init(g.vs.r, t);
     auto row0 = [&](int tt) { return (tt < nsink ? tt : tlo + tt - nsink) * KT; };
     auto load = [&](int tt) {
         const int r0 = row0(tt);
-        sk.load(kb_ + (long long)r0 * g.ks.r, g.ks.r, r0, len, g.D, t);
-        sv.load(vb + (long long)r0 * g.vs.r, g.vs.r, r0, len, g.D, t);
+        sk.load(kb_ + (long long)r0 * g.ks.r, len - r0, g.D, t);
+        sv.load(vb + (long long)r0 * g.vs.r, len - r0, g.D, t);
     };
     if (nt > 0) {
         load(0);
         sk.template put<PREC>(Kimg, t);
         sv.template put<PREC>(Vimg, t);
     }
+    wa_settle(qp);
     __syncthreads();
     for (int tt = 0; tt < nt; ++tt) {
         const int cur = tt & 1, j0 = row0(tt);
         const unsigned char *Kc = Kimg + cur * IMG, *Vc = Vimg + cur * IMG;
         if (tt + 1 < nt) load(tt + 1);
-        if (live && j0 <= whi && (j0 + KT > wlo || j0 < g.sinks)) {
-            f32x16 acc[SUB];
+        if (live) {
+            // the subtiles that hold a key of this wave's window, or a sink
+            auto holds = [&](int jj) { return jj <= whi && (jj + 32 > wlo || jj < far); };
+            auto whole = [&](int jj, int n) { return jj + n <= len && jj + n - 1 <= q0 + g.right && (jj >= q0 + 31 - g.left || jj + n <= g.sinks); };
 #pragma unroll
-            for (int s = 0; s < SUB; ++s) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) acc[s][r] = 0.f;
-#pragma unroll
-                for (int kb = 0; kb < DP / 16; ++kb) {
-                    uint4 ak[NP];
-                    wa_rowfrag<PREC, DP, KT>(Kc, 32 * s + j, h, kb, ak);
-                    mm_mac<PREC>(ak, qp[kb], acc[s]);
-                }
-            }
-            if (!(j0 + KT <= len && j0 + KT - 1 <= q0 + g.right && (j0 >= q0 + 31 - g.left || j0 + KT <= g.sinks))) {
-#pragma unroll
-                for (int s = 0; s < SUB; ++s)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const int jj = j0 + 32 * s + at_drow(r, h);
-                        const bool ok = jj < len && jj <= qi + g.right && (jj >= qi - g.left || jj < g.sinks);
-                        acc[s][r] = ok ? acc[s][r] : -__builtin_inff();
-                    }
-            }
-            float tmax = acc[0][0];
-#pragma unroll
-            for (int s = 0; s < SUB; ++s)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, acc[s][r]);
-            tmax = wa_max32(tmax);
-            if (__ballot(tmax > m + thr) != 0ull) {
-                const float m_new = fmaxf(m, tmax), mc_new = m_new == -__builtin_inff() ? 0.f : m_new * g.c;
-                const float sc = m == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(mc - mc_new);
-                m = m_new;
-                mc = mc_new;
-                l *= sc;
-#pragma unroll
-                for (int d = 0; d < ND; ++d)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) O[d][r] *= sc;
-            }
-#pragma unroll
-            for (int s = 0; s < SUB; ++s) {
-                float pd[16];
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    pd[r] = __builtin_amdgcn_exp2f(fmaf(acc[s][r], g.c, -mc));
-                    l += pd[r];
-                }
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    uint4 pp[NP], av[NP];
-                    at_regfrag<PREC>(pd, ks, pp);
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) {
-                        wa_trfrag<PREC, DP, KT>(Vc + 32 * s * ROWB, lane, d, ks, av);
-                        mm_mac<PREC>(av, pp, O[d]);
-                    }
-                }
-            }
+            for (int s = 0; s < 32 * SUB; s += 32)
+                if (holds(j0 + s))
+                    wa_fwd_tile<T, DP, 1>(Kc + s * ROWB, Vc + s * ROWB, j0 + s, lane, g.c, thr, whole(j0 + s, 32), lo, hi, far, qp, m, mc, l, O);
         }
         if (tt + 1 < nt) { sk.template put<PREC>(Kimg + (cur ^ 1) * IMG, t); sv.template put<PREC>(Vimg + (cur ^ 1) * IMG, t); }
         __syncthreads();
@@ -339,19 +397,26 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
     const int tlo = max(0, qa - g.left) / KT, thi = min(len - 1, qb + g.right) / KT;
     const int nsink = min((min(g.sinks, len) + KT - 1) / KT, tlo);
     const int nt = qa < len ? nsink + thi - tlo + 1 : 0;
-    const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right);
+    const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right), far = min(g.sinks, len);
+    const int hi = mine ? min(len - 1, qi + g.right) : -1, lo = mine ? min(qi - g.left, hi + 1) : 0;      // rows behind the length see nothing
     WaStage<T, DP, KT, 256> sk, sv;
+    sk.init(g.ks.r, t);
+    sv.init(g.vs.r, t);
     auto row0 = [&](int tt) { return (tt < nsink ? tt : tlo + tt - nsink) * KT; };
     auto load = [&](int tt) {
         const int r0 = row0(tt);
-        sk.load(kb_ + (long long)r0 * g.ks.r, g.ks.r, r0, len, g.D, t);
-        sv.load(vb + (long long)r0 * g.vs.r, g.vs.r, r0, len, g.D, t);
+        sk.load(kb_ + (long long)r0 * g.ks.r, len - r0, g.D, t);
+        sv.load(vb + (long long)r0 * g.vs.r, len - r0, g.D, t);
     };
     if (nt > 0) {
         load(0);
         sk.template put<PREC>(Kimg, t);
         sv.template put<PREC>(Vimg, t);
     }
+    wa_settle(qp);
+    wa_settle(gp);
+    float Lw = Lq;
+    asm volatile("" : "+v"(Lw));
     __syncthreads();
     for (int tt = 0; tt < nt; ++tt) {
         const int cur = tt & 1, j0 = row0(tt);
@@ -371,14 +436,11 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
             }
             float ds[16];
 #pragma unroll
-            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(acc[r], g.c, -Lq)) * (dp[r] - dl);
-            if (!(j0 + KT <= len && q0 + 32 <= len && j0 + KT - 1 <= q0 + g.right && (j0 >= q0 + 31 - g.left || j0 + KT <= g.sinks))) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int jj = j0 + at_drow(r, h);
-                    const bool ok = mine && jj < len && jj <= qi + g.right && (jj >= qi - g.left || jj < g.sinks);
-                    ds[r] = ok ? ds[r] : 0.f;
-                }
+            for (int r = 0; r < 16; ++r) ds[r] = __builtin_amdgcn_exp2f(fmaf(acc[r], g.c, -Lw)) * (dp[r] - dl);
+            if (!(j0 + KT <= len && q0 + 32 <= len && j0 + KT - 1 <= q0 + g.right && (j0 >= q0 + 31 - g.left || j0 + KT <= g.sinks)))
+            {
+                if (j0 >= far) wa_mask<false>(j0, h, lo, hi, 0, 0.f, ds);
+                else wa_mask<true>(j0, h, lo, hi, min(far, hi + 1), 0.f, ds);
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
@@ -408,7 +470,7 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
 
 // one 32-query tile against the wave's 32 keys: K += dS^T q, V += P^T dout (unscaled).  SINK: pairs beyond the window (j < sinks,
 // j < i - left), otherwise the window's
-template <class T, int PREC, int DP, bool SINK>
+template <class T, int PREC, int DP, int R, bool SINK>
 __device__ __forceinline__ void wa_dkv_tile(const WaArgs &g, const unsigned char *Qc, const unsigned char *Gc, const float *Ls, const float *Ds,
                                             int p0, int k0, int len, int lane, const uint4 (&kp)[DP / 16][Mx<PREC>::NP],
                                             const uint4 (&vp)[DP / 16][Mx<PREC>::NP], f32x16 (&AK)[DP / 32], f32x16 (&AV)[DP / 32])
@@ -421,8 +483,8 @@ __device__ __forceinline__ void wa_dkv_tile(const WaArgs &g, const unsigned char
 #pragma unroll
     for (int kb = 0; kb < DP / 16; ++kb) {
         uint4 aq[NP], ag[NP];
-        wa_rowfrag<PREC, DP, 32>(Qc, j, h, kb, aq);
-        wa_rowfrag<PREC, DP, 32>(Gc, j, h, kb, ag);
+        wa_rowfrag<PREC, DP, R>(Qc, j, h, kb, aq);
+        wa_rowfrag<PREC, DP, R>(Gc, j, h, kb, ag);
         mm_mac<PREC>(aq, kp[kb], acc);
         mm_mac<PREC>(ag, vp[kb], dp);
     }
@@ -440,13 +502,11 @@ __device__ __forceinline__ void wa_dkv_tile(const WaArgs &g, const unsigned char
     const bool whole = SINK ? p0 + 32 <= len && k0 + 32 <= min(g.sinks, len) && k0 + 31 < p0 - g.left
                             : p0 + 32 <= len && k0 + 32 <= len && k0 + 31 <= p0 + g.right && k0 >= p0 + 31 - g.left;
     if (!whole) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int i = p0 + at_drow(r, h);
-            const bool ok = i < len && ki < len && (SINK ? ki < g.sinks && ki < i - g.left : ki <= i + g.right && ki >= i - g.left);
-            pd[r] = ok ? pd[r] : 0.f;
-            ds[r] = ok ? ds[r] : 0.f;
-        }
+        // rows that see the lane's key: ki - right <= i <= ki + left, or those beyond the window of a sink
+        const bool on = ki < len && (!SINK || ki < g.sinks);
+        const int hi = !on ? -1 : SINK ? len - 1 : min(len - 1, ki + g.left), lo = !on ? 0 : min(SINK ? ki + g.left + 1 : ki - g.right, hi + 1);
+        wa_mask<false>(p0, h, lo, hi, 0, 0.f, pd);
+        wa_mask<false>(p0, h, lo, hi, 0, 0.f, ds);
     }
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -455,22 +515,23 @@ __device__ __forceinline__ void wa_dkv_tile(const WaArgs &g, const unsigned char
         at_regfrag<PREC>(ds, s, bs);
 #pragma unroll
         for (int d = 0; d < ND; ++d) {
-            wa_trfrag<PREC, DP, 32>(Gc, lane, d, s, af);
+            wa_trfrag<PREC, DP, R>(Gc, lane, d, s, af);
             mm_mac<PREC>(af, bp, AV[d]);
-            wa_trfrag<PREC, DP, 32>(Qc, lane, d, s, af);
+            wa_trfrag<PREC, DP, R>(Qc, lane, d, s, af);
             mm_mac<PREC>(af, bs, AK[d]);
         }
     }
 }
 
 // ------------------------------------------------------------------ backward, key side: dK, dV
+template <class T, int DP> constexpr int WA_QT = Mx<WaT<T>::PB>::NP == 1 ? 64 : 32;      // query rows staged per turn
 template <class T, int DP>
 __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(const WaArgs g, T *__restrict__ dk, T *__restrict__ dv)
 {
-    constexpr int PREC = WaT<T>::PB, NP = Mx<PREC>::NP, IMG = NP * 32 * WaImg<DP>::ROWB, ND = DP / 32;
+    constexpr int PREC = WaT<T>::PB, NP = Mx<PREC>::NP, QT = WA_QT<T, DP>, IMG = NP * QT * WaImg<DP>::ROWB, ND = DP / 32, ROWB = WaImg<DP>::ROWB;
     extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
     unsigned char *Qimg = at_smem, *Gimg = at_smem + 2 * IMG;
-    float (*Ls)[32] = reinterpret_cast<float (*)[32]>(at_smem + 4 * IMG), (*Ds)[32] = Ls + 2;       // [2][32] each
+    float (*Ls)[QT] = reinterpret_cast<float (*)[QT]>(at_smem + 4 * IMG), (*Ds)[QT] = Ls + 2;       // [2][QT] each
     const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     const unsigned bid = wa_order(blockIdx.x, gridDim.x);
     const int blk = bid % g.nblk, bg = bid / g.nblk, b = bg / g.G, gi = bg % g.G;
@@ -486,29 +547,39 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(cons
 #pragma unroll
         for (int r = 0; r < 16; ++r) { AK[d][r] = 0.f; AV[d][r] = 0.f; }
 
-    const int tlo = max(0, ka - g.right) / 32, thi = min(len - 1, kz + g.left) / 32, per = thi - tlo + 1;
-    const int nt = ka < len ? per * g.HG : 0;
-    WaStage<T, DP, 32, 256> sq, sg;
+    // turns: (head of the key head, QT rows) with the heads outermost; hd, rt: of the turn to be loaded
+    const int tlo = max(0, ka - g.right) / QT, thi = min(len - 1, kz + g.left) / QT, nt = ka < len ? (thi - tlo + 1) * g.HG : 0;
+    int hd = 0, rt = tlo, p0 = tlo * QT;
+    WaStage<T, DP, QT, 256> sq, sg;
+    sq.init(g.qs.r, t);
+    sg.init(g.gs.r, t);
     float l1 = 0.f;
-    auto load = [&](int tt) {
-        const int head = gi * g.HG + tt / per, r0 = (tlo + tt % per) * 32;
-        sq.load((const T *)g.q + b * g.qs.b + (long long)r0 * g.qs.r + head * g.qs.h, g.qs.r, r0, len, g.D, t);
-        sg.load((const T *)g.dout + b * g.gs.b + (long long)r0 * g.gs.r + head * g.gs.h, g.gs.r, r0, len, g.D, t);
-        if (t < 64) l1 = r0 + (t & 31) < len ? (t < 32 ? g.lse : g.delta)[((size_t)b * g.H + head) * g.N + r0 + (t & 31)] : 0.f;
+    auto load = [&]() {
+        const int head = gi * g.HG + hd, r0 = rt * QT;
+        sq.load((const T *)g.q + b * g.qs.b + (long long)r0 * g.qs.r + head * g.qs.h, len - r0, g.D, t);
+        sg.load((const T *)g.dout + b * g.gs.b + (long long)r0 * g.gs.r + head * g.gs.h, len - r0, g.D, t);
+        if (t < 2 * QT) l1 = r0 + t % QT < len ? (t < QT ? g.lse : g.delta)[((size_t)b * g.H + head) * g.N + r0 + t % QT] : 0.f;
+        if (++rt > thi) { rt = tlo; ++hd; }
     };
     auto put = [&](int buf) {
         sq.template put<PREC>(Qimg + buf * IMG, t);
         sg.template put<PREC>(Gimg + buf * IMG, t);
-        if (t < 64) (t < 32 ? Ls : Ds)[buf][t & 31] = l1;
+        if (t < 2 * QT) (t < QT ? Ls : Ds)[buf][t % QT] = l1;
     };
-    if (nt > 0) { load(0); put(0); }
+    if (nt > 0) { load(); put(0); }
+    wa_settle(kp);
+    wa_settle(vp);
     __syncthreads();
     for (int tt = 0; tt < nt; ++tt) {
-        const int cur = tt & 1, p0 = (tlo + tt % per) * 32;
-        if (tt + 1 < nt) load(tt + 1);
-        if (k0 < len && p0 + 31 >= k0 - g.right && p0 <= k0 + 31 + g.left)
-            wa_dkv_tile<T, PREC, DP, false>(g, Qimg + cur * IMG, Gimg + cur * IMG, Ls[cur], Ds[cur], p0, k0, len, lane, kp, vp, AK, AV);
+        const int cur = tt & 1, pn = rt * QT;
+        if (tt + 1 < nt) load();
+#pragma unroll
+        for (int s = 0; s < QT; s += 32)
+            if (k0 < len && p0 + s < len && p0 + s + 31 >= k0 - g.right && p0 + s <= k0 + 31 + g.left)
+                wa_dkv_tile<T, PREC, DP, QT, false>(g, Qimg + cur * IMG + s * ROWB, Gimg + cur * IMG + s * ROWB, Ls[cur] + s, Ds[cur] + s, p0 + s, k0, len,
+                                                    lane, kp, vp, AK, AV);
         if (tt + 1 < nt) put(cur ^ 1);
+        p0 = pn;
         __syncthreads();
     }
     if (kt < g.nst) {                                     // the sinks' share from rows beyond their window, chunk by chunk
@@ -560,20 +631,24 @@ __global__ void __launch_bounds__(64 * (WA_SINK_NW<T, DP>), 1) wa_bwd_sink_kerne
 
     const int tlo = min(len, k0 + g.left + 1) / 32, per = (len + 31) / 32 - tlo;               // row tiles that hold i > k0 + left
     const int total = max(per, 0) * g.HG, each = (total + g.nchunk - 1) / g.nchunk, f0 = chunk * each, f1 = min(total, f0 + each);
+    wa_settle(kp);
+    wa_settle(vp);
     for (int f = f0; f < f1; f += NW) {                                                         // trip count is the workgroup's
         const int ff = f + wv;
         const bool on = ff < f1;
         const int head = gi * g.HG + (on ? ff / per : 0), p0 = on ? (tlo + ff % per) * 32 : 0;
         if (on) {
             WaStage<T, DP, 32, 64> sq, sg;
-            sq.load((const T *)g.q + b * g.qs.b + (long long)p0 * g.qs.r + head * g.qs.h, g.qs.r, p0, len, g.D, lane);
-            sg.load((const T *)g.dout + b * g.gs.b + (long long)p0 * g.gs.r + head * g.gs.h, g.gs.r, p0, len, g.D, lane);
+            sq.init(g.qs.r, lane);
+            sg.init(g.gs.r, lane);
+            sq.load((const T *)g.q + b * g.qs.b + (long long)p0 * g.qs.r + head * g.qs.h, len - p0, g.D, lane);
+            sg.load((const T *)g.dout + b * g.gs.b + (long long)p0 * g.gs.r + head * g.gs.h, len - p0, g.D, lane);
             sq.template put<PREC>(Qimg, lane);
             sg.template put<PREC>(Gimg, lane);
             (lane < 32 ? Ls : Ds)[j] = p0 + j < len ? (lane < 32 ? g.lse : g.delta)[((size_t)b * g.H + head) * g.N + p0 + j] : 0.f;
         }
         __syncthreads();
-        if (on) wa_dkv_tile<T, PREC, DP, true>(g, Qimg, Gimg, Ls, Ds, p0, k0, len, lane, kp, vp, AK, AV);
+        if (on) wa_dkv_tile<T, PREC, DP, 32, true>(g, Qimg, Gimg, Ls, Ds, p0, k0, len, lane, kp, vp, AK, AV);
         __syncthreads();
     }
     float *sum = reinterpret_cast<float *>(at_smem);                                            // [dK | dV][channel][key]
@@ -778,6 +853,7 @@ int wa_check(const char *who, const gfs3d_window_attn_args *a)
     for (int n = 0; n < 4; ++n) {
         if (!pt[n]) continue;
         GFS3D_REQUIRE(((uintptr_t)pt[n] & 15) == 0, "%s: a tensor is not aligned to 16 bytes", who);
+        GFS3D_REQUIRE(st[n][1] <= (1 << 23), "%s: rows more than 2^23 elements apart", who);        // 32-bit offsets within a tile
         for (int e = 0; e < 3; ++e) GFS3D_REQUIRE(st[n][e] >= 0 && st[n][e] % gran == 0, "%s: a stride is negative or not a multiple of 16 bytes", who);
     }
     return GFS3D_OK;
@@ -829,7 +905,8 @@ template <class T, int DP> int wa_forward(WaArgs g, void *out, hipStream_t st, c
 template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *dv, hipStream_t st, const char *who)
 {
     constexpr int NP = Mx<WaT<T>::PB>::NP;
-    constexpr size_t img = (size_t)NP * 32 * WaImg<DP>::ROWB, lds = 4 * img, ldk = lds + 4 * 32 * sizeof(float);
+    constexpr int QT = WA_QT<T, DP>;
+    constexpr size_t img = (size_t)NP * 32 * WaImg<DP>::ROWB, lds = 4 * img, ldk = 4 * (img * QT / 32 + QT * sizeof(float));
     const size_t ub = ((size_t)((g.N + 31) / 32) * g.HG + 3) / 4, kb = ((size_t)g.N + 127) / 128;
     GFS3D_REQUIRE(ub * g.B * g.G < (1ull << 31), "%s: %zu workgroups", who, ub * g.B * g.G);
     GFS3D_ENSURE_LDS((wa_bwd_dq_kernel<T, DP>), lds, who);

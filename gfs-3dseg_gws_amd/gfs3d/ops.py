@@ -1489,7 +1489,7 @@ def _heads4(t: torch.Tensor) -> torch.Tensor:
     """A (B, rows, heads, D) tensor as the attention kernels read it: dense channels, strides and address in 16 bytes; a copy where
     they are not (one pass over the tensor)."""
     s, gran = t.stride(), 16 // t.element_size()
-    if s[3] == 1 and s[0] % gran == 0 and s[1] % gran == 0 and s[2] % gran == 0 and t.data_ptr() % 16 == 0:
+    if s[3] == 1 and s[0] % gran == 0 and s[1] % gran == 0 and s[1] <= 1 << 23 and s[2] % gran == 0 and t.data_ptr() % 16 == 0:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
