@@ -26,11 +26,11 @@ struct WaArgs {
     WaStride qs, ks, vs, gs;                      // gs: dout
     const int *lengths;                           // (B) device, or NULL: all S
     float *lse, *delta;                           // (B, H, N): log2-sum-exp2 of the scaled scores; dout . out
-    float *part;                                  // partial sums (sinks' gradients / split keys)
+    float *part, *part2;                          // partial sums: sinks' gradients / split keys; split rows of dK, dV
     int B, N, S, H, G, HG, D;                     // N query rows, S keys per sequence
     int left, right, sinks;
     int nblk;                                     // workgroups per (sequence, key head)
-    int nst, nchunk;                              // sinks' key tiles, row chunks of their gradient
+    int nst, nchunk, nsplit;                      // sinks' key tiles, row chunks of their gradient; row chunks of dK, dV
     float scale, c;                               // c = scale log2(e)
 };
 
@@ -524,6 +524,8 @@ __device__ __forceinline__ void wa_dkv_tile(const WaArgs &g, const unsigned char
 }
 
 // ------------------------------------------------------------------ backward, key side: dK, dV
+// The turns of a workgroup - (head of the key head, QT rows), heads outermost - are dealt to nsplit workgroups where there would be too
+// few; they leave fp32 sums in part2[chunk][dK | dV][B N G D] for wa_bwd_join_kernel.
 template <class T, int DP> constexpr int WA_QT = Mx<WaT<T>::PB>::NP == 1 ? 64 : 32;      // query rows staged per turn
 template <class T, int DP>
 __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(const WaArgs g, T *__restrict__ dk, T *__restrict__ dv)
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(cons
     float (*Ls)[QT] = reinterpret_cast<float (*)[QT]>(at_smem + 4 * IMG), (*Ds)[QT] = Ls + 2;       // [2][QT] each
     const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     const unsigned bid = wa_order(blockIdx.x, gridDim.x);
-    const int blk = bid % g.nblk, bg = bid / g.nblk, b = bg / g.G, gi = bg % g.G;
+    const int chunk = bid % g.nsplit, blk = bid / g.nsplit % g.nblk, bg = bid / g.nsplit / g.nblk, b = bg / g.G, gi = bg % g.G;
     const int len = wa_length(g.lengths, b, g.N), kt = blk * 4 + wv, k0 = kt * 32, ki = k0 + j;
     const int ka = blk * 128, kz = min(ka + 127, len - 1);
 
@@ -547,9 +549,9 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(cons
 #pragma unroll
         for (int r = 0; r < 16; ++r) { AK[d][r] = 0.f; AV[d][r] = 0.f; }
 
-    // turns: (head of the key head, QT rows) with the heads outermost; hd, rt: of the turn to be loaded
-    const int tlo = max(0, ka - g.right) / QT, thi = min(len - 1, kz + g.left) / QT, nt = ka < len ? (thi - tlo + 1) * g.HG : 0;
-    int hd = 0, rt = tlo, p0 = tlo * QT;
+    const int tlo = max(0, ka - g.right) / QT, thi = min(len - 1, kz + g.left) / QT, per = thi - tlo + 1, all = ka < len ? per * g.HG : 0;
+    const int t0 = (int)((long long)all * chunk / g.nsplit), nt = (int)((long long)all * (chunk + 1) / g.nsplit) - t0;
+    int hd = nt > 0 ? t0 / per : 0, rt = nt > 0 ? tlo + t0 % per : 0, p0 = rt * QT;       // hd, rt: of the turn to be loaded next
     WaStage<T, DP, QT, 256> sq, sg;
     sq.init(g.qs.r, t);
     sg.init(g.gs.r, t);
@@ -582,28 +584,62 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(cons
         p0 = pn;
         __syncthreads();
     }
-    if (kt < g.nst) {                                     // the sinks' share from rows beyond their window, chunk by chunk
+    if (g.nsplit == 1 && kt < g.nst) {                        // the sinks' share from rows beyond their window
         const float *pt = g.part + ((size_t)bg * g.nst + kt) * g.nchunk * (2 * DP * 32) + j;
-        for (int ch = 0; ch < g.nchunk; ++ch, pt += 2 * DP * 32)
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+        for (int d = 0; d < ND; ++d) {
+            float x[32];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    AK[d][r] += pt[(32 * d + at_drow(r, h)) * 32];
-                    AV[d][r] += pt[(DP + 32 * d + at_drow(r, h)) * 32];
-                }
+            for (int r = 0; r < 16; ++r) {
+                x[r] = pt[(32 * d + at_drow(r, h)) * 32];
+                x[16 + r] = pt[(DP + 32 * d + at_drow(r, h)) * 32];
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) { AK[d][r] += x[r]; AV[d][r] += x[16 + r]; }
+        }
     }
     if (ki < g.N) {
-        const size_t o = (((size_t)b * g.N + ki) * g.G + gi) * g.D;
+        const size_t o = (((size_t)b * g.N + ki) * g.G + gi) * g.D, all_ = (size_t)g.B * g.N * g.G * g.D;
+        float *pk = g.nsplit > 1 ? g.part2 + (size_t)chunk * 2 * all_ + o : nullptr;
 #pragma unroll
         for (int d = 0; d < ND; ++d)
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const int ch = 32 * d + at_drow(r, h);
                 if (ch >= g.D) continue;
-                wa_store4<T>(dk + o + ch, AK[d][r] * g.scale, AK[d][r + 1] * g.scale, AK[d][r + 2] * g.scale, AK[d][r + 3] * g.scale);
-                wa_store4<T>(dv + o + ch, AV[d][r], AV[d][r + 1], AV[d][r + 2], AV[d][r + 3]);
+                const f32x16 &K = AK[d], &V = AV[d];
+                if (pk) {
+                    wa_store4<float>(pk + ch, K[r], K[r + 1], K[r + 2], K[r + 3]);
+                    wa_store4<float>(pk + all_ + ch, V[r], V[r + 1], V[r + 2], V[r + 3]);
+                } else {
+                    wa_store4<T>(dk + o + ch, K[r] * g.scale, K[r + 1] * g.scale, K[r + 2] * g.scale, K[r + 3] * g.scale);
+                    wa_store4<T>(dv + o + ch, V[r], V[r + 1], V[r + 2], V[r + 3]);
+                }
             }
+    }
+}
+// dK, dV = the chunks' sums in order, then the sinks' share; a thread takes four channels
+template <class T, int DP>
+__global__ void __launch_bounds__(256) wa_bwd_join_kernel(const WaArgs g, T *__restrict__ dk, T *__restrict__ dv)
+{
+    const size_t all = (size_t)g.B * g.N * g.G * g.D, e = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (e >= all) return;
+    const int ch = (int)(e % g.D);
+    const size_t row = e / g.D;
+    const int gi = (int)(row % g.G), ki = (int)(row / g.G % g.N), b = (int)(row / g.G / g.N);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < g.nsplit; ++c) {
+            const float4 x = *reinterpret_cast<const float4 *>(g.part2 + ((size_t)2 * c + w) * all + e);
+            a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+        }
+        if (ki < 32 * g.nst) {
+            const float *pt = g.part + ((size_t)(b * g.G + gi) * g.nst + ki / 32) * g.nchunk * (2 * DP * 32) + (w * DP + ch) * 32 + ki % 32;
+            a.x += pt[0]; a.y += pt[32]; a.z += pt[64]; a.w += pt[96];
+        }
+        const float f = w ? 1.f : g.scale;
+        wa_store4<T>((w ? dv : dk) + e, a.x * f, a.y * f, a.z * f, a.w * f);
     }
 }
 
@@ -667,6 +703,20 @@ __global__ void __launch_bounds__(64 * (WA_SINK_NW<T, DP>), 1) wa_bwd_sink_kerne
     }
     float *o = g.part + (size_t)blockIdx.x * (2 * DP * 32);
     for (int e = t; e < 2 * DP * 32; e += 64 * NW) o[e] = sum[e];
+}
+
+// the chunks of a sink tile added, in order, into the first: thread = 4 values, grid (values / 1024, tiles)
+template <int DP> __global__ void __launch_bounds__(256) wa_sink_sum_kernel(float *__restrict__ part, int nchunk)
+{
+    constexpr int PER = 2 * DP * 32;
+    float4 *p = reinterpret_cast<float4 *>(part + (size_t)blockIdx.y * nchunk * PER) + blockIdx.x * 256 + threadIdx.x;
+    float4 a = p[0];
+#pragma unroll 8
+    for (int c = 1; c < nchunk; ++c) {
+        const float4 x = p[(size_t)c * (PER / 4)];
+        a.x += x.x; a.y += x.y; a.z += x.z; a.w += x.w;
+    }
+    p[0] = a;
 }
 
 // ------------------------------------------------------------------ the last T positions of cached sequences
@@ -880,6 +930,16 @@ void wa_sink_plan(WaArgs &g)
     const long long tiles = (long long)((g.N + 31) / 32) * g.HG;
     g.nchunk = (int)(tiles / 8 < 1 ? 1 : tiles / 8 > 32 ? 32 : tiles / 8);
 }
+// dK, dV: workgroups of 128 keys, their turns split until every CU has two workgroups (at most 8 ways, 4 turns at least)
+void wa_dkv_plan(WaArgs &g, bool most = false)       // most: the bound over all types and reaches
+{
+    const long long blocks = (long long)g.B * g.G * ((g.N + 127) / 128);
+    const long long reach = g.N < 127ll + g.left + g.right ? g.N : 127ll + g.left + g.right, turns = (reach + 63) / 64 * g.HG;
+    long long n = (512 + blocks - 1) / blocks;
+    if (!most && n > turns / 4) n = turns / 4;
+    g.nsplit = (int)(n < 1 ? 1 : n > 8 ? 8 : n);
+}
+size_t wa_split_floats(const WaArgs &g) { return g.nsplit > 1 ? (size_t)g.nsplit * 2 * g.B * g.N * g.G * g.D : 0; }
 size_t wa_sink_floats(const WaArgs &g) { return (size_t)g.B * g.G * g.nst * g.nchunk * 2 * wa_dp(g.D) * 32; }
 void wa_step_plan(WaArgs &g)
 {
@@ -902,15 +962,29 @@ template <class T, int DP> int wa_forward(WaArgs g, void *out, hipStream_t st, c
     GFS3D_LAUNCH_CHECK("wa_fwd_kernel");
     return GFS3D_OK;
 }
+template <class T, int DP> int wa_backward_keys(WaArgs g, void *dk, void *dv, hipStream_t st, const char *who)
+{
+    constexpr int QT = WA_QT<T, DP>;
+    constexpr size_t lds = 4 * ((size_t)Mx<WaT<T>::PB>::NP * QT * WaImg<DP>::ROWB + QT * sizeof(float));
+    g.nblk = (g.N + 127) / 128;
+    const size_t blocks = (size_t)g.nblk * g.B * g.G * g.nsplit;
+    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
+    GFS3D_ENSURE_LDS((wa_bwd_dkv_kernel<T, DP>), lds, who);
+    hipLaunchKernelGGL((wa_bwd_dkv_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), lds, st, g, (T *)dk, (T *)dv);
+    GFS3D_LAUNCH_CHECK("wa_bwd_dkv_kernel");
+    if (g.nsplit > 1) {
+        const size_t threads = (size_t)g.B * g.N * g.G * g.D / 4;
+        hipLaunchKernelGGL((wa_bwd_join_kernel<T, DP>), dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, g, (T *)dk, (T *)dv);
+        GFS3D_LAUNCH_CHECK("wa_bwd_join_kernel");
+    }
+    return GFS3D_OK;
+}
 template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *dv, hipStream_t st, const char *who)
 {
-    constexpr int NP = Mx<WaT<T>::PB>::NP;
-    constexpr int QT = WA_QT<T, DP>;
-    constexpr size_t img = (size_t)NP * 32 * WaImg<DP>::ROWB, lds = 4 * img, ldk = 4 * (img * QT / 32 + QT * sizeof(float));
-    const size_t ub = ((size_t)((g.N + 31) / 32) * g.HG + 3) / 4, kb = ((size_t)g.N + 127) / 128;
+    constexpr size_t img = (size_t)Mx<WaT<T>::PB>::NP * 32 * WaImg<DP>::ROWB, lds = 4 * img;
+    const size_t ub = ((size_t)((g.N + 31) / 32) * g.HG + 3) / 4;
     GFS3D_REQUIRE(ub * g.B * g.G < (1ull << 31), "%s: %zu workgroups", who, ub * g.B * g.G);
     GFS3D_ENSURE_LDS((wa_bwd_dq_kernel<T, DP>), lds, who);
-    GFS3D_ENSURE_LDS((wa_bwd_dkv_kernel<T, DP>), ldk, who);
     g.nblk = (int)ub;
     hipLaunchKernelGGL((wa_bwd_dq_kernel<T, DP>), dim3((unsigned)(ub * g.B * g.G)), dim3(256), lds, st, g, (T *)dq);
     GFS3D_LAUNCH_CHECK("wa_bwd_dq_kernel");
@@ -922,11 +996,14 @@ template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *d
         GFS3D_ENSURE_LDS((wa_bwd_sink_kernel<T, DP>), lsk, who);
         hipLaunchKernelGGL((wa_bwd_sink_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lsk, st, g);
         GFS3D_LAUNCH_CHECK("wa_bwd_sink_kernel");
+        if (g.nchunk > 1) {
+            const size_t tiles = (size_t)g.B * g.G * g.nst;
+            GFS3D_REQUIRE(tiles < 65536, "%s: %zu sink tiles", who, tiles);
+            hipLaunchKernelGGL((wa_sink_sum_kernel<DP>), dim3(2 * DP * 32 / 1024, (unsigned)tiles), dim3(256), 0, st, g.part, g.nchunk);
+            GFS3D_LAUNCH_CHECK("wa_sink_sum_kernel");
+        }
     }
-    g.nblk = (int)kb;
-    hipLaunchKernelGGL((wa_bwd_dkv_kernel<T, DP>), dim3((unsigned)(kb * g.B * g.G)), dim3(256), ldk, st, g, (T *)dk, (T *)dv);
-    GFS3D_LAUNCH_CHECK("wa_bwd_dkv_kernel");
-    return GFS3D_OK;
+    return wa_backward_keys<T, DP>(g, dk, dv, st, who);
 }
 template <class T, int DP> int wa_step(const WaArgs &g, void *out, hipStream_t st, const char *who)
 {
@@ -972,7 +1049,8 @@ extern "C" size_t gfs3d_window_attn_workspace_bytes(int B, int N, int S, int H, 
         return g.nchunk > 1 ? (size_t)B * G * g.nblk * g.nchunk * (64 + wa_dp(D) * 32) * sizeof(float) : 0;
     }
     wa_sink_plan(g);
-    return (align_up((size_t)B * H * N, 64) + wa_sink_floats(g)) * sizeof(float);
+    wa_dkv_plan(g, true);
+    return (align_up((size_t)B * H * N, 64) + wa_sink_floats(g) + wa_split_floats(g)) * sizeof(float);
 }
 
 extern "C" int gfs3d_window_attn_forward(const gfs3d_window_attn_args *a, void *stream)
@@ -993,6 +1071,7 @@ extern "C" int gfs3d_window_attn_backward(const gfs3d_window_attn_args *a, void 
     GFS3D_REQUIRE(a->lse && a->dout && a->dq && a->dk && a->dv && a->workspace, "%s: NULL buffer", who);
     WaArgs g = wa_args(a);
     wa_sink_plan(g);
+    wa_dkv_plan(g);
     const size_t need = gfs3d_window_attn_workspace_bytes(a->B, a->N, a->S, a->H, a->G, a->D, a->left, a->sinks, 0);
     if (a->workspace_bytes < need) {
         set_error("%s: workspace too small (%zu, needs %zu)", who, a->workspace_bytes, need);
@@ -1000,6 +1079,7 @@ extern "C" int gfs3d_window_attn_backward(const gfs3d_window_attn_args *a, void 
     }
     g.delta = (float *)a->workspace;
     g.part = g.delta + align_up((size_t)a->B * a->H * a->N, 64);
+    g.part2 = g.part + wa_sink_floats(g);
     hipStream_t st = static_cast<hipStream_t>(stream);
     WA_DISPATCH((wa_backward<T, DP>(g, a->dq, a->dk, a->dv, st, who)))
 }
