@@ -192,6 +192,32 @@ __device__ __forceinline__ unsigned wa_order(unsigned id, unsigned total)
 }
 constexpr float WA_LAZY = 8.f;        // the running maximum may lag the true one by 2^8: p, its sum and its products stay in range in fp32 and half
 
+// A wave's 32 x DP result (C/D registers: column = row of the output, registers = channels) to memory in whole 16-byte pieces of
+// rows, through the wave's own part of LDS: straight from the registers a row would be written in 8-byte pieces by two lanes
+template <class T, int DP> constexpr int WA_OUT = 32 * (DP * (int)sizeof(T) + 16);
+template <class T, int DP>
+__device__ __forceinline__ void wa_store_rows(unsigned char *lds, const f32x16 (&X)[DP / 32], float f, int lane, T *out, size_t stride, int rows, int D)
+{
+    constexpr int RB = DP * (int)sizeof(T) + 16, V = 16 / (int)sizeof(T), PR = DP / V, RPI = 64 / PR;
+    const int j = lane & 31, h = lane >> 5;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+            wa_store4<T>(reinterpret_cast<T *>(lds + j * RB) + 32 * d + at_drow(r, h), X[d][r] * f, X[d][r + 1] * f, X[d][r + 2] * f, X[d][r + 3] * f);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");       // LDS serves a wave in order
+    __builtin_amdgcn_wave_barrier();
+    const int ch = lane % PR * V;
+#pragma unroll
+    for (int n = 0; n < 32 / RPI; ++n) {
+        const int row = n * RPI + lane / PR;
+        const uint4 x = *reinterpret_cast<const uint4 *>(lds + row * RB + lane % PR * 16);
+        if (row < rows && ch < D) *reinterpret_cast<uint4 *>(out + row * stride + ch) = x;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Hides what the lane does not see among the 32 rows from j0 on in its C/D registers: x[r] = fill unless row j = j0 + at_drow(r, h)
 // has lo <= j <= hi, or j < far (FAR: the sinks the lane sees).  One unsigned comparison per element for the window (hi >= lo - 1).
 template <bool FAR, class X> __device__ __forceinline__ void wa_mask(int j0, int h, int lo, int hi, int far, float fill, X &x)
@@ -272,8 +298,8 @@ __device__ __forceinline__ void wa_fwd_tile(const unsigned char *Kc, const unsig
         }
     }
 }
-template <class T, int DP>
-__global__ void __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4 ? 3 : 4) wa_fwd_kernel(const WaArgs g, T *__restrict__ out)
+template <class T, int DP, int NW>
+__global__ void __launch_bounds__(64 * NW, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4 ? 3 : 4) wa_fwd_kernel(const WaArgs g, T *__restrict__ out)
 {
     constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, KT = WaT<T>::KT, SUB = KT / 32, IMG = NP * KT * WaImg<DP>::ROWB;
     constexpr int ROWB = WaImg<DP>::ROWB, ND = DP / 32;
@@ -283,9 +309,9 @@ __global__ void __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : si
     const unsigned bid = wa_order(blockIdx.x, gridDim.x);
     const int blk = bid % g.nblk, bg = bid / g.nblk, b = bg / g.G, gi = bg % g.G;
     const int len = wa_length(g.lengths, b, g.N), nqt = (g.N + 31) / 32;
-    const int u = blk * 4 + wv, qt = u / g.HG, head = gi * g.HG + u % g.HG, q0 = qt * 32, qi = q0 + j;
+    const int u = blk * NW + wv, qt = u / g.HG, head = gi * g.HG + u % g.HG, q0 = qt * 32, qi = q0 + j;
     const bool live = q0 < len;                         // this wave has rows (qt < nqt follows)
-    const int qa = blk * 4 / g.HG * 32, qb = min((blk * 4 + 3) / g.HG, nqt - 1) * 32 + 31;       // the workgroup's rows
+    const int qa = blk * NW / g.HG * 32, qb = min((blk * NW + NW - 1) / g.HG, nqt - 1) * 32 + 31;       // the workgroup's rows
     const T *kb_ = (const T *)g.k + b * g.ks.b + gi * g.ks.h, *vb = (const T *)g.v + b * g.vs.b + gi * g.vs.h;
 
     uint4 qp[DP / 16][NP];
@@ -303,7 +329,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : si
     const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right), far = min(g.sinks, len);
     const int hi = min(len - 1, qi + g.right), lo = min(qi - g.left, hi + 1);
     const float thr = WA_LAZY / g.c;
-    WaStage<T, DP, KT, 256> sk, sv;
+    WaStage<T, DP, KT, 64 * NW> sk, sv;
     sk.init(g.ks.r, t);
     sv.init(g.vs.r, t);
     auto row0 = [&](int tt) { return (tt < nsink ? tt : tlo + tt - nsink) * KT; };
@@ -335,17 +361,10 @@ __global__ void __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : si
         if (tt + 1 < nt) { sk.template put<PREC>(Kimg + (cur ^ 1) * IMG, t); sv.template put<PREC>(Vimg + (cur ^ 1) * IMG, t); }
         __syncthreads();
     }
-    if (qi < g.N && qt < nqt) {
-        const float lt = wa_sum32(l), inv = lt > 0.f && qi < len ? 1.f / lt : (lt != lt ? lt : 0.f);
-        T *ob = out + (((size_t)b * g.N + qi) * g.H + head) * g.D;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int ch = 32 * d + at_drow(r, h);
-                if (ch < g.D) wa_store4<T>(ob + ch, O[d][r] * inv, O[d][r + 1] * inv, O[d][r + 2] * inv, O[d][r + 3] * inv);
-            }
-        if (g.lse && h == 0) g.lse[((size_t)b * g.H + head) * g.N + qi] = lt > 0.f && qi < len ? mc + __builtin_amdgcn_logf(lt) : __builtin_inff();
+    const float lt = wa_sum32(l), inv = lt > 0.f && qi < len ? 1.f / lt : (lt != lt ? lt : 0.f);
+    if (qt < nqt) {
+        wa_store_rows<T, DP>(at_smem + wv * WA_OUT<T, DP>, O, inv, lane, out + (((size_t)b * g.N + q0) * g.H + head) * g.D, (size_t)g.H * g.D, g.N - q0, g.D);
+        if (qi < g.N && g.lse && h == 0) g.lse[((size_t)b * g.H + head) * g.N + qi] = lt > 0.f && qi < len ? mc + __builtin_amdgcn_logf(lt) : __builtin_inff();
     }
 }
 
@@ -353,6 +372,7 @@ __global__ void __launch_bounds__(256, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : si
 template <class T, int DP>
 __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_bwd_dq_kernel(const WaArgs g, T *__restrict__ dq)
 {
+    constexpr int NW = 4;
     constexpr int PREC = WaT<T>::PB, NP = Mx<PREC>::NP, KT = 32, IMG = NP * KT * WaImg<DP>::ROWB, ND = DP / 32;
     extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
     unsigned char *Kimg = at_smem, *Vimg = at_smem + 2 * IMG;
@@ -360,9 +380,9 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
     const unsigned bid = wa_order(blockIdx.x, gridDim.x);
     const int blk = bid % g.nblk, bg = bid / g.nblk, b = bg / g.G, gi = bg % g.G;
     const int len = wa_length(g.lengths, b, g.N), nqt = (g.N + 31) / 32;
-    const int u = blk * 4 + wv, qt = u / g.HG, head = gi * g.HG + u % g.HG, q0 = qt * 32, qi = q0 + j;
+    const int u = blk * NW + wv, qt = u / g.HG, head = gi * g.HG + u % g.HG, q0 = qt * 32, qi = q0 + j;
     const bool live = q0 < len, mine = qi < len;
-    const int qa = blk * 4 / g.HG * 32, qb = min((blk * 4 + 3) / g.HG, nqt - 1) * 32 + 31;
+    const int qa = blk * NW / g.HG * 32, qb = min((blk * NW + NW - 1) / g.HG, nqt - 1) * 32 + 31;
     const T *kb_ = (const T *)g.k + b * g.ks.b + gi * g.ks.h, *vb = (const T *)g.v + b * g.vs.b + gi * g.vs.h;
 
     uint4 qp[DP / 16][NP], gp[DP / 16][NP];
@@ -399,7 +419,7 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
     const int nt = qa < len ? nsink + thi - tlo + 1 : 0;
     const int wlo = max(0, q0 - g.left), whi = min(len - 1, q0 + 31 + g.right), far = min(g.sinks, len);
     const int hi = mine ? min(len - 1, qi + g.right) : -1, lo = mine ? min(qi - g.left, hi + 1) : 0;      // rows behind the length see nothing
-    WaStage<T, DP, KT, 256> sk, sv;
+    WaStage<T, DP, KT, 64 * NW> sk, sv;
     sk.init(g.ks.r, t);
     sv.init(g.vs.r, t);
     auto row0 = [&](int tt) { return (tt < nsink ? tt : tlo + tt - nsink) * KT; };
@@ -456,17 +476,10 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
         if (tt + 1 < nt) { sk.template put<PREC>(Kimg + (cur ^ 1) * IMG, t); sv.template put<PREC>(Vimg + (cur ^ 1) * IMG, t); }
         __syncthreads();
     }
-    if (qi < g.N && qt < nqt) {
-        T *ob = dq + (((size_t)b * g.N + qi) * g.H + head) * g.D;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int ch = 32 * d + at_drow(r, h);
-                if (ch < g.D) wa_store4<T>(ob + ch, A[d][r] * g.scale, A[d][r + 1] * g.scale, A[d][r + 2] * g.scale, A[d][r + 3] * g.scale);
-            }
-    }
+    if (qt < nqt)
+        wa_store_rows<T, DP>(at_smem + wv * WA_OUT<T, DP>, A, g.scale, lane, dq + (((size_t)b * g.N + q0) * g.H + head) * g.D, (size_t)g.H * g.D, g.N - q0, g.D);
 }
+
 
 // one 32-query tile against the wave's 32 keys: K += dS^T q, V += P^T dout (unscaled).  SINK: pairs beyond the window (j < sinks,
 // j < i - left), otherwise the window's
@@ -598,24 +611,17 @@ __global__ void __launch_bounds__(256, DP == 128 ? 1 : 2) wa_bwd_dkv_kernel(cons
             for (int r = 0; r < 16; ++r) { AK[d][r] += x[r]; AV[d][r] += x[16 + r]; }
         }
     }
-    if (ki < g.N) {
-        const size_t o = (((size_t)b * g.N + ki) * g.G + gi) * g.D, all_ = (size_t)g.B * g.N * g.G * g.D;
-        float *pk = g.nsplit > 1 ? g.part2 + (size_t)chunk * 2 * all_ + o : nullptr;
-#pragma unroll
-        for (int d = 0; d < ND; ++d)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const int ch = 32 * d + at_drow(r, h);
-                if (ch >= g.D) continue;
-                const f32x16 &K = AK[d], &V = AV[d];
-                if (pk) {
-                    wa_store4<float>(pk + ch, K[r], K[r + 1], K[r + 2], K[r + 3]);
-                    wa_store4<float>(pk + all_ + ch, V[r], V[r + 1], V[r + 2], V[r + 3]);
-                } else {
-                    wa_store4<T>(dk + o + ch, K[r] * g.scale, K[r + 1] * g.scale, K[r + 2] * g.scale, K[r + 3] * g.scale);
-                    wa_store4<T>(dv + o + ch, V[r], V[r + 1], V[r + 2], V[r + 3]);
-                }
-            }
+    if (k0 < g.N) {
+        const size_t o = (((size_t)b * g.N + k0) * g.G + gi) * g.D, row = (size_t)g.G * g.D, all_ = (size_t)g.B * g.N * g.G * g.D;
+        unsigned char *lds = at_smem + wv * WA_OUT<float, DP>;
+        if (g.nsplit > 1) {
+            float *pk = g.part2 + (size_t)chunk * 2 * all_ + o;
+            wa_store_rows<float, DP>(lds, AK, 1.f, lane, pk, row, g.N - k0, g.D);
+            wa_store_rows<float, DP>(lds, AV, 1.f, lane, pk + all_, row, g.N - k0, g.D);
+        } else {
+            wa_store_rows<T, DP>(lds, AK, g.scale, lane, dk + o, row, g.N - k0, g.D);
+            wa_store_rows<T, DP>(lds, AV, 1.f, lane, dv + o, row, g.N - k0, g.D);
+        }
     }
 }
 // dK, dV = the chunks' sums in order, then the sinks' share; a thread takes four channels
@@ -951,21 +957,46 @@ void wa_step_plan(WaArgs &g)
     if (n > tiles / (2 * NW)) n = tiles / (2 * NW);
     g.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
-template <class T, int DP> int wa_forward(WaArgs g, void *out, hipStream_t st, const char *who)
+// Waves of a workgroup in the forward: eight share every staged key tile where that leaves four workgroups to a CU (rooms of 2 x 65536 x
+// 8 heads x 64: 405 us, with four waves 422; dQ in eight waves spills at four waves per SIMD: 659 us for 561), four otherwise
+template <class T, int DP> bool wa_wide(const WaArgs &g)
 {
-    constexpr size_t lds = 4ull * Mx<WaT<T>::PF>::NP * WaT<T>::KT * WaImg<DP>::ROWB;
-    g.nblk = (int)(((long long)((g.N + 31) / 32) * g.HG + 3) / 4);
+    return sizeof(T) == 2 && DP <= 64 && (long long)g.B * g.G * (((g.N + 31) / 32 * (long long)g.HG + 7) / 8) >= 1024;
+}
+template <class T, int DP, int NW> int wa_forward_queries(WaArgs g, void *out, hipStream_t st, const char *who)
+{
+    constexpr size_t im = 4ull * Mx<WaT<T>::PF>::NP * WaT<T>::KT * WaImg<DP>::ROWB, ou = (size_t)NW * WA_OUT<T, DP>, lds = im > ou ? im : ou;
+    g.nblk = (int)(((long long)((g.N + 31) / 32) * g.HG + NW - 1) / NW);
     const size_t blocks = (size_t)g.B * g.G * g.nblk;
     GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
-    GFS3D_ENSURE_LDS((wa_fwd_kernel<T, DP>), lds, who);
-    hipLaunchKernelGGL((wa_fwd_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), lds, st, g, (T *)out);
+    GFS3D_ENSURE_LDS((wa_fwd_kernel<T, DP, NW>), lds, who);
+    hipLaunchKernelGGL((wa_fwd_kernel<T, DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)out);
     GFS3D_LAUNCH_CHECK("wa_fwd_kernel");
+    return GFS3D_OK;
+}
+template <class T, int DP> int wa_forward(const WaArgs &g, void *out, hipStream_t st, const char *who)
+{
+    if constexpr (sizeof(T) == 2 && DP <= 64) {
+        if (wa_wide<T, DP>(g)) return wa_forward_queries<T, DP, 8>(g, out, st, who);
+    }
+    return wa_forward_queries<T, DP, 4>(g, out, st, who);
+}
+template <class T, int DP> int wa_backward_queries(WaArgs g, void *dq, hipStream_t st, const char *who)
+{
+    constexpr int NW = 4;
+    constexpr size_t im = 4ull * Mx<WaT<T>::PB>::NP * 32 * WaImg<DP>::ROWB, ou = (size_t)NW * WA_OUT<T, DP>, lds = im > ou ? im : ou;
+    g.nblk = (int)(((long long)((g.N + 31) / 32) * g.HG + NW - 1) / NW);
+    const size_t blocks = (size_t)g.B * g.G * g.nblk;
+    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
+    GFS3D_ENSURE_LDS((wa_bwd_dq_kernel<T, DP>), lds, who);
+    hipLaunchKernelGGL((wa_bwd_dq_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)dq);
+    GFS3D_LAUNCH_CHECK("wa_bwd_dq_kernel");
     return GFS3D_OK;
 }
 template <class T, int DP> int wa_backward_keys(WaArgs g, void *dk, void *dv, hipStream_t st, const char *who)
 {
     constexpr int QT = WA_QT<T, DP>;
-    constexpr size_t lds = 4 * ((size_t)Mx<WaT<T>::PB>::NP * QT * WaImg<DP>::ROWB + QT * sizeof(float));
+    constexpr size_t im = 4 * ((size_t)Mx<WaT<T>::PB>::NP * QT * WaImg<DP>::ROWB + QT * sizeof(float)), ou = 4ull * WA_OUT<float, DP>, lds = im > ou ? im : ou;
     g.nblk = (g.N + 127) / 128;
     const size_t blocks = (size_t)g.nblk * g.B * g.G * g.nsplit;
     GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
@@ -981,13 +1012,8 @@ template <class T, int DP> int wa_backward_keys(WaArgs g, void *dk, void *dv, hi
 }
 template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *dv, hipStream_t st, const char *who)
 {
-    constexpr size_t img = (size_t)Mx<WaT<T>::PB>::NP * 32 * WaImg<DP>::ROWB, lds = 4 * img;
-    const size_t ub = ((size_t)((g.N + 31) / 32) * g.HG + 3) / 4;
-    GFS3D_REQUIRE(ub * g.B * g.G < (1ull << 31), "%s: %zu workgroups", who, ub * g.B * g.G);
-    GFS3D_ENSURE_LDS((wa_bwd_dq_kernel<T, DP>), lds, who);
-    g.nblk = (int)ub;
-    hipLaunchKernelGGL((wa_bwd_dq_kernel<T, DP>), dim3((unsigned)(ub * g.B * g.G)), dim3(256), lds, st, g, (T *)dq);
-    GFS3D_LAUNCH_CHECK("wa_bwd_dq_kernel");
+    constexpr size_t img = (size_t)Mx<WaT<T>::PB>::NP * 32 * WaImg<DP>::ROWB;
+    if (int rc = wa_backward_queries<T, DP>(g, dq, st, who)) return rc;
     if (g.nst > 0) {
         constexpr int NW = (WA_SINK_NW<T, DP>);
         constexpr size_t ws = (size_t)NW * (2 * img + 256), sum = 2ull * DP * 32 * sizeof(float), lsk = ws > sum ? ws : sum;
