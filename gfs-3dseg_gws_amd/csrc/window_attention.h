@@ -729,15 +729,18 @@ template <int DP> __global__ void __launch_bounds__(256) wa_sink_sum_kernel(floa
 // Columns of a wave's tile = up to 32 (head of the key head, row) pairs, so that a cached key is read once for all of them.  The
 // visible key tiles of a sequence are dealt to the waves of its nchunk workgroups in turn; each wave keeps its own running
 // softmax, the waves of a workgroup join through LDS, the workgroups (nchunk > 1) through part[..][m | l | O] and a second kernel.
-template <class T, int DP> constexpr int WA_STEP_NW = sizeof(T) == 4 && DP == 128 ? 4 : 8;
-template <class T, int DP>
-__global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP>), 1) wa_step_kernel(const WaArgs g, T *__restrict__ out)
+// HBM-bound: a wave has two tiles of K and V in flight (32 keys x 128 channels: 32 KB).  WIDE: up to 16 waves of one workgroup share
+// short caches, which saves the second launch; otherwise 4, so that workgroups at different stages share a CU.
+template <class T, int DP, bool WIDE> constexpr int WA_STEP_NW = !WIDE ? 4 : sizeof(T) == 4 ? (DP == 128 ? 4 : 8) : DP == 128 ? 8 : 16;
+template <class T, int DP, bool WIDE>
+__global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4 && DP == 128 ? 1 : 2) wa_step_kernel(const WaArgs g, T *__restrict__ out)
 {
-    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, IMG = NP * 32 * WaImg<DP>::ROWB, ND = DP / 32, NK = DP / 16, NW = (WA_STEP_NW<T, DP>);
+    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, IMG = NP * 32 * WaImg<DP>::ROWB, ND = DP / 32, NK = DP / 16, NW = (WA_STEP_NW<T, DP, WIDE>);
     extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
     const int t = threadIdx.x, lane = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), j = lane & 31, h = lane >> 5;
     unsigned char *Vimg = at_smem + wv * IMG;
-    const int sp = blockIdx.x % g.nchunk, cb = blockIdx.x / g.nchunk % g.nblk, bg = blockIdx.x / g.nchunk / g.nblk, b = bg / g.G, gi = bg % g.G;
+    const unsigned bid = wa_order(blockIdx.x, gridDim.x);        // the heads of a sequence lie side by side: on one XCD
+    const int sp = bid % g.nchunk, cb = bid / g.nchunk % g.nblk, bg = bid / g.nchunk / g.nblk, b = bg / g.G, gi = bg % g.G;
     const int len = wa_length(g.lengths, b, g.S), col = cb * 32 + j, hs = col / g.N, head = gi * g.HG + hs, tq = col % g.N, qi = len - g.N + tq;
     const bool mine = hs < g.HG && qi >= 0;
     const T *kb_ = (const T *)g.k + b * g.ks.b + gi * g.ks.h, *vb = (const T *)g.v + b * g.vs.b + gi * g.vs.h;
@@ -826,43 +829,41 @@ __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP>), 1) wa_step_kernel(co
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
-    // join the waves: [wave][m, l][32] then [channel][32] sums in wave order
+    // join the waves: ml[wave][m, l][32], o[wave][channel][32]; every thread sums its values over the waves in order
     l = wa_sum32(l);
     const float mb = m == -__builtin_inff() ? -__builtin_inff() : mc;      // maximum in base-2 units
     __syncthreads();
     float *ml = reinterpret_cast<float *>(at_smem), *osum = ml + NW * 64;
     if (h == 0) { ml[wv * 64 + j] = mb; ml[wv * 64 + 32 + j] = l; }
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) osum[(wv * DP + 32 * d + at_drow(r, h)) * 32 + j] = O[d][r];
     __syncthreads();
-    float M = -__builtin_inff(), Lt = 0.f;
+    float M = -__builtin_inff(), Lt = 0.f, f[NW];                          // (thread t's column is j as well: t & 31)
+#pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, ml[w * 64 + j]);
+#pragma unroll
     for (int w = 0; w < NW; ++w) {
         const float mw = ml[w * 64 + j];
-        Lt += mw == -__builtin_inff() ? ml[w * 64 + 32 + j] : ml[w * 64 + 32 + j] * __builtin_amdgcn_exp2f(mw - M);
-    }
-    const float f = mb == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(mb - M);      // a wave without keys holds zeros
-    for (int w = 0; w < NW; ++w) {
-        if (wv == w) {
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float *a = osum + (32 * d + at_drow(r, h)) * 32 + j;
-                    *a = w ? fmaf(O[d][r], f, *a) : O[d][r] * f;
-                }
-        }
-        __syncthreads();
-    }
-    if (g.nchunk > 1) {
-        float *o = g.part + (size_t)blockIdx.x * (64 + DP * 32);
-        if (wv == 0 && h == 0) { o[j] = M; o[32 + j] = Lt; }
-        for (int e = t; e < DP * 32; e += 64 * NW) o[64 + e] = osum[e];
-        return;
+        f[w] = mw == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(mw - M);      // a wave without keys holds zeros
+        Lt = fmaf(ml[w * 64 + 32 + j], f[w], Lt);
     }
     const float inv = Lt > 0.f ? 1.f / Lt : (Lt != Lt ? Lt : 0.f);
-    if (hs < g.HG)
-        for (int ch = 4 * (t >> 5); ch < g.D; ch += 8 * NW)
-            wa_store4<T>(out + (((size_t)b * g.N + tq) * g.H + head) * g.D + ch, osum[ch * 32 + j] * inv, osum[(ch + 1) * 32 + j] * inv,
-                         osum[(ch + 2) * 32 + j] * inv, osum[(ch + 3) * 32 + j] * inv);
+    float *po = g.part + (size_t)bid * (64 + DP * 32);
+    if (g.nchunk > 1 && t < 32) { po[j] = M; po[32 + j] = Lt; }
+    for (int ch = 4 * (t >> 5); ch < DP; ch += 8 * NW) {
+        float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(osum[(w * DP + ch + e) * 32 + j], f[w], o[e]);
+        if (g.nchunk > 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) po[64 + (ch + e) * 32 + j] = o[e];
+        } else if (hs < g.HG && ch < g.D)
+            wa_store4<T>(out + (((size_t)b * g.N + tq) * g.H + head) * g.D + ch, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+    }
 }
 
 // joins the nchunk partial softmaxes of one (sequence, key head, 32 columns): thread = (column, 4 channels)
@@ -947,14 +948,16 @@ void wa_dkv_plan(WaArgs &g, bool most = false)       // most: the bound over all
 }
 size_t wa_split_floats(const WaArgs &g) { return g.nsplit > 1 ? (size_t)g.nsplit * 2 * g.B * g.N * g.G * g.D : 0; }
 size_t wa_sink_floats(const WaArgs &g) { return (size_t)g.B * g.G * g.nst * g.nchunk * 2 * wa_dp(g.D) * 32; }
-void wa_step_plan(WaArgs &g)
+// Short caches, or as many sequences as CUs twice over: one workgroup each (wide, no second launch); else the keys are split until there
+// are four workgroups to a CU, four tiles to a wave at least
+void wa_step_plan(WaArgs &g, bool &wide)
 {
-    const int NW = 8;
     g.nblk = (int)(((long long)g.HG * g.N + 31) / 32);
     const long long keys = (long long)g.left + g.N < g.S ? (long long)g.left + g.N : g.S;
     const long long tiles = keys / 32 + 2 + (g.sinks + 31) / 32, blocks = (long long)g.B * g.G * g.nblk;
-    long long n = (512 + blocks - 1) / blocks;
-    if (n > tiles / (2 * NW)) n = tiles / (2 * NW);
+    wide = tiles <= 64;
+    long long n = wide ? 1 : (1024 + blocks - 1) / blocks;
+    if (n > tiles / 16) n = tiles / 16;
     g.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 // Waves of a workgroup in the forward: eight share every staged key tile where that leaves four workgroups to a CU (rooms of 2 x 65536 x
@@ -1031,20 +1034,25 @@ template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *d
     }
     return wa_backward_keys<T, DP>(g, dk, dv, st, who);
 }
-template <class T, int DP> int wa_step(const WaArgs &g, void *out, hipStream_t st, const char *who)
+template <class T, int DP, bool WIDE> int wa_step_go(const WaArgs &g, void *out, hipStream_t st, const char *who)
 {
-    constexpr int NW = (WA_STEP_NW<T, DP>);
-    constexpr size_t im = (size_t)NW * Mx<WaT<T>::PF>::NP * 32 * WaImg<DP>::ROWB, js = (size_t)(NW * 64 + DP * 32) * sizeof(float), lds = im > js ? im : js;
+    constexpr int NW = (WA_STEP_NW<T, DP, WIDE>);
+    constexpr size_t im = (size_t)NW * Mx<WaT<T>::PF>::NP * 32 * WaImg<DP>::ROWB, js = (size_t)NW * (64 + DP * 32) * sizeof(float), lds = im > js ? im : js;
+    static_assert(lds <= 160 * 1024, "LDS");
     const size_t groups = (size_t)g.B * g.G * g.nblk, blocks = groups * g.nchunk;
     GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
-    GFS3D_ENSURE_LDS((wa_step_kernel<T, DP>), lds, who);
-    hipLaunchKernelGGL((wa_step_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)out);
+    GFS3D_ENSURE_LDS((wa_step_kernel<T, DP, WIDE>), lds, who);
+    hipLaunchKernelGGL((wa_step_kernel<T, DP, WIDE>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)out);
     GFS3D_LAUNCH_CHECK("wa_step_kernel");
     if (g.nchunk > 1) {
         hipLaunchKernelGGL((wa_join_kernel<T, DP>), dim3((unsigned)groups), dim3(256), 0, st, g, (T *)out);
         GFS3D_LAUNCH_CHECK("wa_join_kernel");
     }
     return GFS3D_OK;
+}
+template <class T, int DP> int wa_step(const WaArgs &g, bool wide, void *out, hipStream_t st, const char *who)
+{
+    return wide ? wa_step_go<T, DP, true>(g, out, st, who) : wa_step_go<T, DP, false>(g, out, st, who);
 }
 
 // one call per (type, padded head size)
@@ -1071,7 +1079,8 @@ extern "C" size_t gfs3d_window_attn_workspace_bytes(int B, int N, int S, int H, 
     g.B = B; g.N = N; g.S = S; g.H = H; g.G = G; g.HG = H / G; g.D = D;
     g.left = left < S ? left : S; g.sinks = sinks < S ? sinks : S;
     if (step) {
-        wa_step_plan(g);
+        bool wide;
+        wa_step_plan(g, wide);
         return g.nchunk > 1 ? (size_t)B * G * g.nblk * g.nchunk * (64 + wa_dp(D) * 32) * sizeof(float) : 0;
     }
     wa_sink_plan(g);
@@ -1116,7 +1125,8 @@ extern "C" int gfs3d_window_attn_step(const gfs3d_window_attn_args *a, void *str
     if (int rc = wa_check(who, a)) return rc;
     GFS3D_REQUIRE(a->lengths, "%s: NULL lengths", who);
     WaArgs g = wa_args(a);
-    wa_step_plan(g);
+    bool wide;
+    wa_step_plan(g, wide);
     const size_t need = gfs3d_window_attn_workspace_bytes(a->B, a->N, a->S, a->H, a->G, a->D, a->left, a->sinks, 1);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need)) {
         set_error("%s: workspace too small (%zu, needs %zu)", who, a->workspace_bytes, need);
@@ -1124,5 +1134,5 @@ extern "C" int gfs3d_window_attn_step(const gfs3d_window_attn_args *a, void *str
     }
     g.part = (float *)a->workspace;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    WA_DISPATCH((wa_step<T, DP>(g, a->out, st, who)))
+    WA_DISPATCH((wa_step<T, DP>(g, wide, a->out, st, who)))
 }

@@ -1630,46 +1630,46 @@ def rotary_frequencies(pairs: int, base: float = 10000.0, scaling: Optional[str]
     return freqs.to(device) if device is not None else freqs, magnitude
 
 
-def _rotary_launch(q, k, positions, freqs, magnitude, interleaved, inverse):
+def _rotary_launch(q, k, positions, axes, freqs, magnitude, interleaved, inverse):
     B, N, H, D = q.shape
     if q.stride(3) != 1:
         q = q.contiguous()
-    qo = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device)
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
     kp, kop, ks, kos, G, ko = None, None, (0, 0, 0), (0, 0, 0), 0, None
     if k is not None:
         if k.stride(3) != 1:
             k = k.contiguous()
         G = k.shape[2]
-        ko = torch.empty((B, N, G, D), dtype=k.dtype, device=k.device)
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
         kp, kop, ks, kos = k.data_ptr(), ko.data_ptr(), k.stride()[:3], (N * G * D, G * D, D)
     if B and N:
         _launch("gfs3d_rotary", q.get_device(), _lib.RotaryArgs(
             B, N, D, _TYPE_IDS[q.dtype], H, G, q.data_ptr(), kp, qo.data_ptr(), kop, q.stride()[:3], ks, (N * H * D, H * D, D), kos,
-            positions.data_ptr(), _POSITION_IDS[positions.dtype], positions.shape[2], freqs.shape[0], interleaved, inverse,
+            positions.data_ptr(), _POSITION_IDS[positions.dtype], axes, freqs.shape[0], interleaved, inverse,
             freqs.data_ptr(), magnitude))
     return qo, ko
 
 
 class RotaryFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, freqs, magnitude, interleaved):
+    def forward(ctx, q, k, positions, axes, freqs, magnitude, interleaved):
         ctx.set_materialize_grads(False)
-        if any(ctx.needs_input_grad[:2]):
-            ctx.save_for_backward(positions, freqs)
-            ctx.cfg = (magnitude, interleaved)
-        return _rotary_launch(q, k, positions, freqs, magnitude, interleaved, 0)
+        ctx.save_for_backward(positions, freqs)
+        ctx.cfg = (magnitude, interleaved)
+        ctx.axes = axes
+        return _rotary_launch(q, k, positions, axes, freqs, magnitude, interleaved, 0)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, freqs = ctx.saved_tensors
         if dq is None and dk is None:
-            return (None,) * 6
+            return (None,) * 7
         if dq is None:
-            gk, gq = _rotary_launch(dk, None, positions, freqs, *ctx.cfg, 1)
+            gk, gq = _rotary_launch(dk, None, positions, ctx.axes, freqs, *ctx.cfg, 1)
         else:
-            gq, gk = _rotary_launch(dq, dk, positions, freqs, *ctx.cfg, 1)
-        return gq, gk, None, None, None, None
+            gq, gk = _rotary_launch(dq, dk, positions, ctx.axes, freqs, *ctx.cfg, 1)
+        return gq, gk, None, None, None, None, None
 
 
 def rotary(q, k, positions, freqs, magnitude: float = 1.0, layout: str = "half"):
@@ -1688,21 +1688,21 @@ def rotary(q, k, positions, freqs, magnitude: float = 1.0, layout: str = "half")
         raise RuntimeError(f"gfs3d.rotary: positions must be an int32, int64 or float32 tensor on {q.device}")
     if positions.dim() == 1:
         positions = positions.expand(B, positions.shape[0])
-    if positions.dim() == 2:
-        positions = positions[:, :, None]
-    if positions.dim() != 3 or tuple(positions.shape[:2]) != (B, N) or not 1 <= positions.shape[2] <= 3:
-        raise RuntimeError(f"gfs3d.rotary: positions must be ({N},), ({B}, {N}) or ({B}, {N}, 1..3), got {tuple(positions.shape)}")
+    ps = positions.shape
+    axes = 1 if len(ps) == 2 else ps[2] if len(ps) == 3 else 0
+    if not 1 <= axes <= 3 or ps[0] != B or ps[1] != N:
+        raise RuntimeError(f"gfs3d.rotary: positions must be ({N},), ({B}, {N}) or ({B}, {N}, 1..3), got {tuple(ps)}")
     if not isinstance(freqs, torch.Tensor) or freqs.dtype is not torch.float64 or freqs.get_device() != device or freqs.dim() != 1:
         raise RuntimeError(f"gfs3d.rotary: freqs must be a 1-d float64 tensor on {q.device}")
-    P = freqs.shape[0]
-    if P < 1 or 2 * P * positions.shape[2] > D or P * positions.shape[2] > 1024 or H < 1 or (k is not None and k.shape[2] < 1):
-        raise RuntimeError(f"gfs3d.rotary: {positions.shape[2]} axes of {P} pairs do not fit heads of {D} channels")
+    P = freqs.shape[0] * axes
+    if P < 1 or 2 * P > D or P > 1024 or H < 1 or (k is not None and k.shape[2] < 1):
+        raise RuntimeError(f"gfs3d.rotary: {axes} axes of {freqs.shape[0]} pairs do not fit heads of {D} channels")
     positions, freqs = positions.contiguous(), freqs.contiguous()
     interleaved = 1 if layout == "interleaved" else 0
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        got = RotaryFunction.apply(q, k, positions, freqs, float(magnitude), interleaved)
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+        got = RotaryFunction.apply(q, k, positions, axes, freqs, float(magnitude), interleaved)
     else:
-        got = _rotary_launch(q, k, positions, freqs, float(magnitude), interleaved, 0)
+        got = _rotary_launch(q, k, positions, axes, freqs, float(magnitude), interleaved, 0)
     return got if k is not None else got[0]
 
 
