@@ -27,7 +27,10 @@ struct RoArgs {
     const double *freqs;
     float magnitude, sign;
     int interleaved, tb;                    // tb: tokens of a workgroup
+    int per;                                // units of a head
+    unsigned m_per, m_heads;                // ceil(2^32 / per), / heads where that divides exactly (0: plain division)
 };
+__device__ __forceinline__ int ro_div(int u, int d, unsigned m) { return m ? (int)__umulhi((unsigned)u, m) : u / d; }
 __device__ __forceinline__ float2 ro_turn(double turns)
 {
     const double z = (turns - __builtin_rint(turns)) * 4.0, nq = __builtin_rint(z);
@@ -43,9 +46,15 @@ template <class T, int VEC>
 __global__ void __launch_bounds__(256) rotary_kernel(const RoArgs g)
 {
     extern __shared__ __attribute__((aligned(16))) float2 ro_cs[];          // [token][axis * pairs + p]
+    __shared__ long long ro_at[16][4];                                      // a token's offset in q, k and their outputs
     const int t = threadIdx.x, AP = g.axes * g.pairs;
     const long long tok0 = (long long)blockIdx.x * g.tb;
     const int nt = (int)min((long long)g.tb, g.tokens - tok0);
+    if (t < 4 * nt) {
+        const long long b = (tok0 + t / 4) / g.N, n = (tok0 + t / 4) % g.N;
+        const int w = t & 1;
+        ro_at[t / 4][t & 3] = t & 2 ? b * g.ob[w] + n * g.orr[w] : b * g.sb[w] + n * g.sr[w];
+    }
     for (int e = t; e < nt * AP; e += 256) {
         const long long tk = tok0 + e / AP;
         const int ap = e % AP, a = ap / g.pairs;
@@ -60,12 +69,13 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RoArgs g)
     const int P = g.pairs, heads = g.heads[0] + g.heads[1];
     if (g.interleaved) {
         constexpr int W = VEC > 1 ? VEC : 2;                                // channels of a unit: whole pairs
-        const int per = (g.D + W - 1) / W, units = nt * heads * per;
+        const int per = g.per, units = nt * heads * per;
+#pragma unroll 4
         for (int u = t; u < units; u += 256) {
-            const int c0 = u % per * W, th = u / per, hd = th % heads, tk = th / heads, w = hd >= g.heads[0], hh = w ? hd - g.heads[0] : hd;
-            const long long b = (tok0 + tk) / g.N, n = (tok0 + tk) % g.N;
-            const T *x = (const T *)g.x[w] + b * g.sb[w] + n * g.sr[w] + hh * g.sh[w] + c0;
-            T *y = (T *)g.y[w] + b * g.ob[w] + n * g.orr[w] + hh * g.oh[w] + c0;
+            const int th = ro_div(u, per, g.m_per), c0 = (u - th * per) * W, tk = ro_div(th, heads, g.m_heads), hd = th - tk * heads;
+            const int w = hd >= g.heads[0], hh = w ? hd - g.heads[0] : hd;
+            const T *x = (const T *)g.x[w] + ro_at[tk][w] + hh * g.sh[w] + c0;
+            T *y = (T *)g.y[w] + ro_at[tk][2 + w] + hh * g.oh[w] + c0;
             typedef T Tw __attribute__((ext_vector_type(W)));
             Tw v;
             if constexpr (VEC > 1) v = *reinterpret_cast<const Tw *>(x);
@@ -92,12 +102,13 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RoArgs g)
         return;
     }
     // half: a unit is VEC pairs of one section, or VEC channels behind the sections
-    const int pu = AP / VEC, ru = (g.D - 2 * AP + VEC - 1) / VEC, per = pu + ru, units = nt * heads * per;
+    const int pu = AP / VEC, per = g.per, units = nt * heads * per;
+#pragma unroll 4
     for (int u = t; u < units; u += 256) {
-        const int k = u % per, th = u / per, hd = th % heads, tk = th / heads, w = hd >= g.heads[0], hh = w ? hd - g.heads[0] : hd;
-        const long long b = (tok0 + tk) / g.N, n = (tok0 + tk) % g.N;
-        const T *x = (const T *)g.x[w] + b * g.sb[w] + n * g.sr[w] + hh * g.sh[w];
-        T *y = (T *)g.y[w] + b * g.ob[w] + n * g.orr[w] + hh * g.oh[w];
+        const int th = ro_div(u, per, g.m_per), k = u - th * per, tk = ro_div(th, heads, g.m_heads), hd = th - tk * heads;
+        const int w = hd >= g.heads[0], hh = w ? hd - g.heads[0] : hd;
+        const T *x = (const T *)g.x[w] + ro_at[tk][w] + hh * g.sh[w];
+        T *y = (T *)g.y[w] + ro_at[tk][2 + w] + hh * g.oh[w];
         if (k < pu) {
             const int ap = k * VEC, ch = ap / P * 2 * P + ap % P;
             Tv a = *reinterpret_cast<const Tv *>(x + ch), c = *reinterpret_cast<const Tv *>(x + ch + P);
@@ -505,6 +516,12 @@ extern "C" int gfs3d_rotary(const gfs3d_rotary_args *a, void *stream)
     g.tb = (int)(want < 1 ? 1 : want > most ? most : want);
     const long long blocks = (g.tokens + g.tb - 1) / g.tb;
     GFS3D_REQUIRE(blocks < (1ll << 31) && (long long)g.tb * (g.heads[0] + g.heads[1]) * a->D < (1ll << 31), "%s: too many values", who);
+    const int V = al ? vec : 1, W = V > 1 ? V : 2, heads = g.heads[0] + g.heads[1];
+    g.per = g.interleaved ? (a->D + W - 1) / W : AP / V + (a->D - 2 * AP + V - 1) / V;
+    const long long units = (long long)g.tb * heads * g.per;             // u < 2^32 / d: the product with the rounded-up reciprocal is exact
+    auto magic = [&](int d) { return d > 1 && units * d < (1ll << 32) ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
+    g.m_per = magic(g.per);
+    g.m_heads = magic(heads);
     hipStream_t st = static_cast<hipStream_t>(stream);
     const size_t lds = (size_t)g.tb * AP * sizeof(float2);
 #define RO_GO(T, V) hipLaunchKernelGGL((rotary_kernel<T, V>), dim3((unsigned)blocks), dim3(256), lds, st, g)
