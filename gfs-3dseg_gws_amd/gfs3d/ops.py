@@ -1474,6 +1474,12 @@ def _no_grad_form(who: str, *tensors) -> None:
         raise RuntimeError(f"gfs3d.{who} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
+def _first_order(who: str) -> None:
+    """In a backward: gradients of gradients (create_graph=True) are refused, not left out."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"gfs3d.{who}: the backward is not differentiable (create_graph=True)")
+
+
 def _launch(fn: str, device: int, args) -> None:
     call = getattr(_lib.lib(), fn)
     if device == torch._C._cuda_getDevice():
@@ -1548,8 +1554,8 @@ class WindowAttentionFunction(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
+        _first_order("window_attention")
         q, k, v, out, lse, lengths = ctx.saved_tensors
         a, _, device = _window_args("window_attention", q, k, v, *ctx.cfg, lengths)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -1572,7 +1578,7 @@ def window_attention(q, k, v, left: Optional[int] = None, right: Optional[int] =
     h // (H // G).  left / right None: unlimited (right = 0: causal).  `lengths` (B,): valid rows of each sequence; what lies behind
     is not read, its outputs and gradients are zero.  Keys and values in front of it have to be finite: a row next to a window takes
     part in products with zero weights.  scale defaults to D ** -0.5.  fp32, bf16 or half; D a multiple of 8 up to 128.
-    Differentiable once, deterministic."""
+    Differentiable once (create_graph is refused), deterministic."""
     return WindowAttentionFunction.apply(q, k, v, left, right, int(sinks), scale, lengths)
 
 
@@ -1660,8 +1666,8 @@ class RotaryFunction(torch.autograd.Function):
         return _rotary_launch(q, k, positions, axes, freqs, magnitude, interleaved, 0)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
+        _first_order("rotary")
         positions, freqs = ctx.saved_tensors
         if dq is None and dk is None:
             return (None,) * 7
@@ -1758,40 +1764,33 @@ class RmsNormFunction(torch.autograd.Function):
         return y if stream is None else (y, stream)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, ds=None):
+        _first_order("rms_norm")
         s, weight, rstd = ctx.saved_tensors
         dtype, eps, has_res = ctx.cfg
-        shape = dy.shape if dy is not None else ds.shape if ds is not None else None
-        if shape is None:
+        if dy is None and ds is None:
             return None, None, None, None
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         if dy is None:
             return ds.to(dtype) if need_x else None, torch.zeros_like(weight) if need_w else None, ds if need_r else None, None
         weight = weight.contiguous()
-        s2, dy2 = _rows2(s), _rows2(dy)
-        a = _lib.RmsNormArgs()
-        a.rows, a.C, a.type, a.eps = s2.shape[0], s2.shape[1], _TYPE_IDS[dtype], eps
-        a.residual_f32, a.weight_f32 = int(s.dtype == torch.float32), int(weight.dtype == torch.float32)
-        wide = has_res and s.dtype != dtype                         # an fp32 stream beside 16-bit x: two gradients
-        dx = torch.empty(shape, dtype=dtype, device=s.device) if need_x or (need_r and not wide) else None
-        dr = torch.empty(shape, dtype=s.dtype, device=s.device) if need_r and wide else None
-        dw = torch.empty_like(weight) if need_w else None
-        if a.rows:
-            a.x, a.x_stride, a.weight, a.rstd = s2.data_ptr(), s2.stride(0), weight.data_ptr(), rstd.data_ptr()
-            a.dy, a.dy_stride = dy2.data_ptr(), dy2.stride(0)
-            if ds is not None:
-                ds2 = _rows2(ds)
-                a.ds, a.ds_stride = ds2.data_ptr(), ds2.stride(0)
-            a.dx = dx.data_ptr() if dx is not None else None
-            a.dresidual = dr.data_ptr() if dr is not None else None
-            if need_w:
-                nbytes = _lib.lib().gfs3d_rms_norm_workspace_bytes(a.rows, a.C)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
-                a.dweight, a.workspace, a.workspace_bytes = dw.data_ptr(), ws.data_ptr(), nbytes
-            _launch("gfs3d_rms_norm_backward", s.get_device(), a)
-        elif need_w:
-            dw.zero_()
+        s2, dy2, ds2 = _rows2(s), _rows2(dy), None if ds is None else _rows2(ds)
+        rows, C = s2.shape
+        wide = has_res and s.dtype is not dtype                     # an fp32 stream beside 16-bit x: two gradients
+        dx = torch.empty_like(dy, memory_format=torch.contiguous_format) if need_x or (need_r and not wide) else None
+        dr = torch.empty_like(s, memory_format=torch.contiguous_format) if need_r and wide else None
+        dw = ws = None
+        nbytes = 0
+        if need_w:
+            dw = torch.empty_like(weight) if rows else torch.zeros_like(weight)
+            nbytes = _lib.lib().gfs3d_rms_norm_workspace_bytes(rows, C)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=s.device)
+        if rows:
+            ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+            _launch("gfs3d_rms_norm_backward", s.get_device(), _lib.RmsNormArgs(
+                rows, C, _TYPE_IDS[dtype], 1 if s.dtype is torch.float32 else 0, 1 if weight.dtype is torch.float32 else 0, 0, 0, eps,
+                s2.data_ptr(), None, weight.data_ptr(), s2.stride(0), 0, None, None, None, rstd.data_ptr(), dy2.data_ptr(), ptr(ds2),
+                dy2.stride(0), 0 if ds2 is None else ds2.stride(0), ptr(dx), ptr(dr), ptr(dw), ptr(ws), nbytes))
         return dx if need_x else None, dw, (dr if wide else dx) if need_r else None, None
 
 
