@@ -20,7 +20,7 @@ import torch.nn.functional as F
 from torch import nn
 
 from gfs3d import ops
-from model.attention import SelfAttention
+from model.attention import attention_learner
 from model.dgcnn import DGCNN, BaseLearner  # noqa: F401  (BaseLearner re-exported like the reference module)
 
 # The reference seeds the global RNGs when this module is imported (capl.py:13-17);
@@ -52,7 +52,7 @@ class mpti_net_Point_GeoAsWeight_v2(nn.Module):
         self.encoder = DGCNN(args.edgeconv_widths, args.dgcnn_mlp_widths, args.pc_in_dim, k=args.dgcnn_k,
                              return_edgeconvs=True)
         self.base_learner = BaseLearner(args.dgcnn_mlp_widths[-1], args.base_widths)
-        self.att_learner = SelfAttention(args.dgcnn_mlp_widths[-1], args.output_dim)
+        self.att_learner = attention_learner(args, args.dgcnn_mlp_widths[-1], args.output_dim)
         self.feat_dim = args.edgeconv_widths[0][-1] + args.output_dim + args.base_widths[-1]
         self.gp = gp
         self.gp.requires_grad = False
@@ -94,13 +94,13 @@ class mpti_net_Point_GeoAsWeight_v2(nn.Module):
         words = self._words_on(x.device)
         if not (x.is_cuda and self._heads_fusable()):
             edge_feats, level2 = self.encoder(x)
-            semantic = torch.cat((edge_feats[0], self.att_learner(level2), self.base_learner(level2)), dim=1)
+            semantic = torch.cat((edge_feats[0], self.att_learner(level2, x), self.base_learner(level2)), dim=1)
             soft, one_hot, word = ops.WordAssignFunction.apply(torch.cat(edge_feats, dim=1), words, _COS_SCALE)
             point_feat = self.fusion(torch.cat([soft, semantic], dim=1))
             return point_feat, semantic, (one_hot if want_onehot else word)
         sync = self.encoder.bn_sync
         edge_feats, edge_pm, level2_pm = self.encoder(x, point_major=True)
-        att = self.att_learner.forward_pm(level2_pm)                                        # (B,64,N)
+        att = self.att_learner.forward_pm(level2_pm, x)                                        # (B,64,N)
         base = self.base_learner.forward_pm(level2_pm, sync=sync, want_cf=want_semantic)
         base_cf, base_pm = base if want_semantic else (None, base)
         conv, bn, act = self.fusion[0], self.fusion[1], self.fusion[2]

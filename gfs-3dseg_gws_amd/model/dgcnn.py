@@ -14,7 +14,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from gfs3d import ops
-from model.attention import SelfAttention
+from model.attention import attention_learner
 
 _LRELU = 0.2
 
@@ -264,7 +264,7 @@ class DGCNNSeg_att(nn.Module):
         super().__init__()
         self.encoder = DGCNN(args.edgeconv_widths, args.dgcnn_mlp_widths, args.pc_in_dim, k=args.dgcnn_k)
         self.base_learner = BaseLearner(args.dgcnn_mlp_widths[-1], args.base_widths)
-        self.att_learner = SelfAttention(args.dgcnn_mlp_widths[-1], args.output_dim)
+        self.att_learner = attention_learner(args, args.dgcnn_mlp_widths[-1], args.output_dim)
         self.feat_dim = args.edgeconv_widths[0][-1] + args.output_dim + args.base_widths[-1]
         self.segmenter = nn.Sequential(
             nn.Conv1d(self.feat_dim, 256, 1, bias=False), nn.BatchNorm1d(256), nn.LeakyReLU(_LRELU),
@@ -276,13 +276,13 @@ class DGCNNSeg_att(nn.Module):
                 and self.att_learner.out_channel == 64 and self.encoder.fully_fused():
             # everything after the EdgeConv blocks on the HIP point-wise kernels, point-major throughout
             feats, feats_pm, level2_pm = self.encoder(pc, point_major=True)
-            att = self.att_learner.forward_pm(level2_pm)
+            att = self.att_learner.forward_pm(level2_pm, pc)
             base_pm = self.base_learner.forward_pm(level2_pm, sync=self.encoder.bn_sync)
             packed = ops.pack_rows([feats_pm[0], att, base_pm], [False, True, False])
             logits = segmenter_forward_pm(self.segmenter, packed, self.training, self.encoder.bn_sync)
             return (logits, feats[0]) if return_feat else logits
         level1, level2 = self.encoder(pc)
-        feat = torch.cat((level1, self.att_learner(level2), self.base_learner(level2)), dim=1)
+        feat = torch.cat((level1, self.att_learner(level2, pc), self.base_learner(level2)), dim=1)
         logits = self.segmenter(feat)
         return (logits, level1) if return_feat else logits
 

@@ -398,3 +398,149 @@ def test_other_streams():
     torch.cuda.synchronize()
     for pair in got:
         assert all(torch.equal(a, b) for a, b in zip(pair, want))
+
+
+def test_window_attention_learner_against_float64():
+    """WindowSelfAttention, two layers, against the float64 forms in the curve's order; its gradients against differences."""
+    from gfs3d.morton import morton_order
+    from model.attention import WindowSelfAttention
+    torch.manual_seed(3)
+    B, N, C = 2, 150, 64
+    m = WindowSelfAttention(C, 32, window=20, sinks=3, layers=2, heads=4, key_heads=2, head_dim=32).cuda()
+    with torch.no_grad():
+        for n in m.norms:
+            n.add_(0.1 * rnd(100, n.shape, torch.float32))
+    x, cloud = rnd(101, (B, C, N), torch.float32).requires_grad_(), rnd(102, (B, 9, N), torch.float32)
+    out = m(x, cloud)
+    order, rank = (t.cpu() for t in morton_order(cloud[:, :3]))
+    d = lambda t: t.detach().cpu().double()  # noqa: E731
+    stream, branch = d(x).transpose(1, 2).gather(1, order[:, :, None].expand(-1, -1, C)), None
+    for norm, qm, om in zip(m.norms, m.qkv_maps, m.out_maps):
+        stream = stream if branch is None else stream + branch
+        y = O.rms(stream, norm, 1e-6, None)["y"][0]
+        qkv = (y @ d(qm.weight).t()).view(B, N, 8, 32)
+        q, k = (O.rotary(t, torch.arange(N), m.freqs, 1.0, "half")[0] for t in (qkv[:, :, :4], qkv[:, :, 4:6]))
+        branch = O.attention(q, k, qkv[:, :, 6:], 20, 20, 3, None)["out"][0].reshape(B, N, -1) @ d(om.weight).t()
+    want = O.rms(stream + branch, m.norms[2], 1e-6, None)["y"][0] @ d(m.head_map.weight).t()
+    want = want.gather(1, rank[:, :, None].expand(-1, -1, 32)).transpose(1, 2)
+    # five fp32 products of 64 to 128 terms and four norms of values of a few units: 128 u32 = 8e-6 each, relative to their terms' sum
+    assert float((d(out) - want).abs().max()) < 2e-4
+    w = rnd(103, out.shape, torch.float32)
+    leaves = [x] + list(m.parameters())
+    grads = torch.autograd.grad(out, leaves, w)
+    assert all(bool(g.isfinite().all()) and bool(g.any()) for g in grads)
+    for n in (0, 1, 4, 6, len(leaves) - 1):
+        t, h = leaves[n], 2.0 ** -7
+        dirn = grads[n] / grads[n].norm()                     # the steepest direction: the slope is the gradient's norm
+        f = []
+        for s in (h, -h):
+            with torch.no_grad():
+                t.add_(s * dirn)
+                f.append(float((m(x, cloud).double() * w.double()).sum()))
+                t.sub_(s * dirn)
+        slope, at = (f[0] - f[1]) / (2 * h), float(grads[n].double().norm())
+        assert abs(slope - at) <= 0.02 * at, (n, slope, at)   # h^2 f''' / 6 of a unit step: below 1e-4 of the slope times the model's curvature
+
+
+def test_models_take_the_window_attention_learner():
+    """args.att_window puts it into both models: training gradients reach its weights, points may be given in any order, and models
+    without the option hold the reference's learner."""
+    import types
+    from model.attention import SelfAttention, WindowSelfAttention
+    from model.dgcnn import DGCNNSeg_att
+    args = types.SimpleNamespace(edgeconv_widths=[[64, 64]] * 3, dgcnn_mlp_widths=[512, 256], pc_in_dim=9, dgcnn_k=20, base_widths=[128, 64],
+                                 output_dim=64, eval_weight=1.2)
+    assert type(DGCNNSeg_att(args, 5).att_learner) is SelfAttention
+    args.att_window, args.att_layers = 64, 2
+    torch.manual_seed(4)
+    net = DGCNNSeg_att(args, 5).cuda().train()
+    assert type(net.att_learner) is WindowSelfAttention and len(net.att_learner.qkv_maps) == 2
+    pc = rnd(104, (2, 9, 512), torch.float32)
+    for mode in ("f32", "bf16"):
+        with ops().compute(mode):
+            net.zero_grad()
+            logits = net(pc)
+            logits.square().mean().backward()
+        assert logits.shape == (2, 5, 512) and bool(logits.isfinite().all())
+        assert all(bool(p.grad.isfinite().all()) and bool(p.grad.any()) for p in net.att_learner.parameters())
+    net.eval()
+    with torch.no_grad():
+        perm = torch.randperm(512, generator=torch.Generator().manual_seed(5)).cuda()
+        a, b = net.att_learner(pc[:, :1].expand(-1, 256, -1), pc), net.att_learner(pc[:, :1, perm].expand(-1, 256, -1), pc[:, :, perm])
+    assert torch.equal(a[:, :, perm], b)                      # random coordinates: no two points on one cell of the curve, or the test's seed is bad
+
+
+def test_entry_points_refuse():
+    o = ops()
+    q = rnd(110, (2, 8, 4, 64), torch.bfloat16)
+    k = q[:, :, :2]
+    f, _ = o.rotary_frequencies(32, device="cuda")
+    pos, lens = torch.arange(8, device="cuda"), torch.tensor([8, 8], device="cuda")
+    x, w = rnd(111, (4, 96), torch.float16), torch.ones(96, device="cuda")
+    for call in (
+            lambda: o.window_attention(q, k.float(), k), lambda: o.window_attention(q, k.cpu(), k), lambda: o.window_attention(q, q[:, :, :3], q[:, :, :3]),
+            lambda: o.window_attention(q, k[:, :5], k[:, :5]), lambda: o.window_attention(q, k, k[:, :, :1]), lambda: o.window_attention(q.int(), k, k),
+            lambda: o.window_attention(q, k, k, left=-1), lambda: o.window_attention(q, k, k, sinks=-1), lambda: o.window_attention(q, k, k, scale=0.0),
+            lambda: o.window_attention(q, k, k, scale=float("inf")), lambda: o.window_attention(q, k, k, lengths=lens.float()),
+            lambda: o.window_attention(q, k, k, lengths=lens.cpu()), lambda: o.window_attention(q, k, k, lengths=lens[:1]),
+            lambda: o.window_attention_step(q, k, k, None), lambda: o.window_attention_step(q.requires_grad_(), k, k, lens),
+            lambda: o.rotary(q, k, pos.double(), f), lambda: o.rotary(q, k, pos[:7], f), lambda: o.rotary(q, k, pos.cpu(), f),
+            lambda: o.rotary(q, k, pos, f.float()), lambda: o.rotary(q, k, pos.view(1, 8, 1).expand(2, 8, 2).contiguous(), f),
+            lambda: o.rotary(q, k.float(), pos, f), lambda: o.rotary(q[0], None, pos, f),
+            lambda: o.rms_norm(x, w[:95]), lambda: o.rms_norm(x, w.double()), lambda: o.rms_norm(x, w.bfloat16()), lambda: o.rms_norm(x, w, -1.0),
+            lambda: o.rms_norm(x, w, residual=x[:3]), lambda: o.rms_norm(x, w, residual=x.bfloat16()), lambda: o.rms_norm_fp8(x, w, group=64),
+            lambda: o.rms_norm_fp8(x, w, group=48), lambda: o.rms_norm_fp8(x, w.clone().requires_grad_())):
+        with pytest.raises(RuntimeError):
+            call()
+    q = q.detach()
+    for call in (lambda: o.window_attention(q[..., :60].contiguous(), k[..., :60].contiguous(), k[..., :60].contiguous()),
+                 lambda: o.rms_norm(torch.zeros((1, 16392), device="cuda"), torch.ones(16392, device="cuda"))):
+        with pytest.raises(NotImplementedError):
+            call()
+    with pytest.raises(ValueError):
+        o.rotary(q, k, pos, f, layout="quarter")
+    a = q.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(o.window_attention(a, k, k).sum(), a, create_graph=True)
+
+
+def test_empty_batches_and_sequences():
+    o = ops()
+    f, _ = o.rotary_frequencies(32, device="cuda")
+    for shape in ((0, 5, 2, 64), (2, 0, 2, 64)):
+        q = torch.zeros(shape, device="cuda", requires_grad=True)
+        out = o.window_attention(q, q, q)
+        assert out.shape == q.shape and torch.autograd.grad(out.sum(), q)[0].shape == q.shape
+        assert o.rotary(q.detach(), None, torch.zeros(shape[:2], dtype=torch.int32, device="cuda"), f).shape == q.shape
+        x = torch.zeros((*shape[:2], 16), device="cuda", requires_grad=True)
+        w = torch.ones(16, device="cuda", requires_grad=True)
+        dx, dw = torch.autograd.grad(o.rms_norm(x, w).sum(), (x, w))
+        assert dx.shape == x.shape and not dw.any()
+    q = torch.ones((2, 1, 2, 64), device="cuda")
+    assert not o.window_attention_step(q, q[:, :0], q[:, :0], torch.zeros(2, dtype=torch.int32, device="cuda")).any()
+
+
+def test_two_captured_steps_share_nothing():
+    """Two captured calls with workspaces of their own, replayed in turn and with eager calls between."""
+    o = ops()
+    lens = [torch.tensor([n], dtype=torch.int32, device="cuda") for n in (9000, 7000)]
+    ins = [[rnd(120 + 3 * i, (1, 1, 4, 64), torch.bfloat16), rnd(121 + 3 * i, (1, 9000, 1, 64), torch.bfloat16), rnd(122 + 3 * i, (1, 9000, 1, 64), torch.bfloat16)] for i in range(2)]
+    want = [o.window_attention_step(*ins[i], lens[i]) for i in range(2)]
+    graphs, outs = [], []
+    for i in range(2):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            o.window_attention_step(*ins[i], lens[i])
+        torch.cuda.current_stream().wait_stream(side)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(o.window_attention_step(*ins[i], lens[i]))
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs:
+            g.replay()
+        again = [o.window_attention_step(*ins[i], lens[i]) for i in range(2)]
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert torch.equal(outs[i], want[i]) and torch.equal(again[i], want[i])
