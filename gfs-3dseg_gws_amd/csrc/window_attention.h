@@ -731,7 +731,7 @@ template <int DP> __global__ void __launch_bounds__(256) wa_sink_sum_kernel(floa
 // softmax, the waves of a workgroup join through LDS, the workgroups (nchunk > 1) through part[..][m | l | O] and a second kernel.
 // HBM-bound: a wave has two tiles of K and V in flight (32 keys x 128 channels: 32 KB).  WIDE: up to 16 waves of one workgroup share
 // short caches, which saves the second launch; otherwise 4, so that workgroups at different stages share a CU.
-template <class T, int DP, bool WIDE> constexpr int WA_STEP_NW = !WIDE ? 4 : sizeof(T) == 4 ? (DP == 128 ? 4 : 8) : DP == 128 ? 8 : 16;
+template <class T, int DP, bool WIDE> constexpr int WA_STEP_NW = !WIDE ? 4 : sizeof(T) == 4 ? (DP == 128 ? 4 : 8) : 8;
 template <class T, int DP, bool WIDE>
 __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4 && DP == 128 ? 1 : 2) wa_step_kernel(const WaArgs g, T *__restrict__ out)
 {
@@ -964,7 +964,7 @@ void wa_step_plan(WaArgs &g, bool &wide)
 // 8 heads x 64: 405 us, with four waves 422; dQ in eight waves spills at four waves per SIMD: 659 us for 561), four otherwise
 template <class T, int DP> bool wa_wide(const WaArgs &g)
 {
-    return sizeof(T) == 2 && DP <= 64 && (long long)g.B * g.G * (((g.N + 31) / 32 * (long long)g.HG + 7) / 8) >= 1024;
+    return sizeof(T) == 2 && (long long)g.B * g.G * (((g.N + 31) / 32 * (long long)g.HG + 7) / 8) >= 1024;
 }
 template <class T, int DP, int NW> int wa_forward_queries(WaArgs g, void *out, hipStream_t st, const char *who)
 {
@@ -979,7 +979,7 @@ template <class T, int DP, int NW> int wa_forward_queries(WaArgs g, void *out, h
 }
 template <class T, int DP> int wa_forward(const WaArgs &g, void *out, hipStream_t st, const char *who)
 {
-    if constexpr (sizeof(T) == 2 && DP <= 64) {
+    if constexpr (sizeof(T) == 2) {
         if (wa_wide<T, DP>(g)) return wa_forward_queries<T, DP, 8>(g, out, st, who);
     }
     return wa_forward_queries<T, DP, 4>(g, out, st, who);

@@ -355,7 +355,7 @@ def test_a_layer_of_them_together_and_replayed():
 
     def step():
         s, y = _layer(o, h, x, w, wqkv, pos, freqs, H, G, D, lengths)
-        return (s, y) + torch.autograd.grad((s + y).square().sum(), (w, wqkv))
+        return (s.detach(), y.detach()) + torch.autograd.grad((s + y).square().sum(), (w, wqkv))
 
     # (no eager graph over w and wqkv may live while a backward through them is captured: torch would make its streams part of the
     # capture, which ends the process)
