@@ -23,6 +23,7 @@ namespace {
 struct WaStride { long long b, r, h; };          // elements between sequences, rows, heads
 struct WaArgs {
     const void *q, *k, *v, *out, *dout;
+    void *low;                                    // (B, N, H, D) what rounding took from out (16-bit types): delta is formed from both
     WaStride qs, ks, vs, gs;                      // gs: dout
     const int *lengths;                           // (B) device, or NULL: all S
     float *lse, *delta;                           // (B, H, N): log2-sum-exp2 of the scaled scores; dout . out
@@ -35,9 +36,11 @@ struct WaArgs {
 };
 
 template <class T> struct WaT;
-template <> struct WaT<float> { static constexpr int PF = PREC_X6, PB = PREC_X6, KT = 32; };
-template <> struct WaT<__bf16> { static constexpr int PF = PREC_BF16, PB = PREC_BF16, KT = 64; };
-template <> struct WaT<_Float16> { static constexpr int PF = PREC_F16, PB = PREC_X3, KT = 64; };
+template <> struct WaT<float> { static constexpr int PF = PREC_X6, PB = PREC_X6; };
+template <> struct WaT<__bf16> { static constexpr int PF = PREC_BF16, PB = PREC_BF16; };
+template <> struct WaT<_Float16> { static constexpr int PF = PREC_F16, PB = PREC_X3; };
+// keys of a staged tile in the forward
+template <class T, int DP, int NW> constexpr int WA_KT = sizeof(T) == 4 ? 32 : NW == 8 && DP == 128 ? 128 : 64;
 
 // eight consecutive channels as they lie in memory
 template <class T> struct WaRaw { uint4 a; };
@@ -235,12 +238,12 @@ template <bool FAR, class X> __device__ __forceinline__ void wa_mask(int j0, int
 
 // ------------------------------------------------------------------ forward
 // NS 32-key subtiles of the staged tile, from Kc / Vc on (keys j0 ..): scores, running softmax, products.  `whole`: every key is seen
-template <class T, int DP, int NS>
+template <class T, int DP, int KT, int NS>
 __device__ __forceinline__ void wa_fwd_tile(const unsigned char *Kc, const unsigned char *Vc, int j0, int lane, float c, float thr, bool whole,
                                             int lo, int hi, int far, const uint4 (&qp)[DP / 16][Mx<WaT<T>::PF>::NP], float &m, float &mc,
                                             float &l, f32x16 (&O)[DP / 32])
 {
-    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, KT = WaT<T>::KT, ROWB = WaImg<DP>::ROWB, ND = DP / 32;
+    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, ROWB = WaImg<DP>::ROWB, ND = DP / 32;
     const int j = lane & 31, h = lane >> 5;
     f32x16 acc[NS];
 #pragma unroll
@@ -301,7 +304,7 @@ __device__ __forceinline__ void wa_fwd_tile(const unsigned char *Kc, const unsig
 template <class T, int DP, int NW>
 __global__ void __launch_bounds__(64 * NW, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) : sizeof(T) == 4 ? 3 : 4) wa_fwd_kernel(const WaArgs g, T *__restrict__ out)
 {
-    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, KT = WaT<T>::KT, SUB = KT / 32, IMG = NP * KT * WaImg<DP>::ROWB;
+    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, KT = (WA_KT<T, DP, NW>), SUB = KT / 32, IMG = NP * KT * WaImg<DP>::ROWB;
     constexpr int ROWB = WaImg<DP>::ROWB, ND = DP / 32;
     extern __shared__ __attribute__((aligned(16))) unsigned char at_smem[];
     unsigned char *Kimg = at_smem, *Vimg = at_smem + 2 * IMG;
@@ -356,14 +359,27 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) 
 #pragma unroll
             for (int s = 0; s < 32 * SUB; s += 32)
                 if (holds(j0 + s))
-                    wa_fwd_tile<T, DP, 1>(Kc + s * ROWB, Vc + s * ROWB, j0 + s, lane, g.c, thr, whole(j0 + s, 32), lo, hi, far, qp, m, mc, l, O);
+                    wa_fwd_tile<T, DP, KT, 1>(Kc + s * ROWB, Vc + s * ROWB, j0 + s, lane, g.c, thr, whole(j0 + s, 32), lo, hi, far, qp, m, mc, l, O);
         }
         if (tt + 1 < nt) { sk.template put<PREC>(Kimg + (cur ^ 1) * IMG, t); sv.template put<PREC>(Vimg + (cur ^ 1) * IMG, t); }
         __syncthreads();
     }
     const float lt = wa_sum32(l), inv = lt > 0.f && qi < len ? 1.f / lt : (lt != lt ? lt : 0.f);
     if (qt < nqt) {
-        wa_store_rows<T, DP>(at_smem + wv * WA_OUT<T, DP>, O, inv, lane, out + (((size_t)b * g.N + q0) * g.H + head) * g.D, (size_t)g.H * g.D, g.N - q0, g.D);
+        const size_t o = (((size_t)b * g.N + q0) * g.H + head) * g.D;
+        wa_store_rows<T, DP>(at_smem + wv * WA_OUT<T, DP>, O, inv, lane, out + o, (size_t)g.H * g.D, g.N - q0, g.D);
+        if constexpr (sizeof(T) == 2) {
+            if (g.low) {
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const float x = O[d][r] * inv;
+                        O[d][r] = x - (float)(T)x;
+                    }
+                wa_store_rows<T, DP>(at_smem + wv * WA_OUT<T, DP>, O, 1.f, lane, (T *)g.low + o, (size_t)g.H * g.D, g.N - q0, g.D);
+            }
+        }
         if (qi < g.N && g.lse && h == 0) g.lse[((size_t)b * g.H + head) * g.N + qi] = lt > 0.f && qi < len ? mc + __builtin_amdgcn_logf(lt) : __builtin_inff();
     }
 }
@@ -390,7 +406,7 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
     float dl = 0.f;
     {
         const T *grow = (const T *)g.dout + b * g.gs.b + (long long)qi * g.gs.r + head * g.gs.h;
-        const T *orow = (const T *)g.out + (((size_t)b * g.N + qi) * g.H + head) * g.D;
+        const T *orow = (const T *)g.out + (((size_t)b * g.N + qi) * g.H + head) * g.D, *lrow = (const T *)g.low + (((size_t)b * g.N + qi) * g.H + head) * g.D;
 #pragma unroll
         for (int kb = 0; kb < DP / 16; ++kb) {
             const int ch = 16 * kb + 8 * h;
@@ -399,6 +415,16 @@ __global__ void __launch_bounds__(256, DP == 128 && sizeof(T) == 4 ? 1 : 2) wa_b
             float fg[8], fo[8];
             wa_floats<T>(rg, fg);
             wa_floats<T>(ro, fo);
+            if constexpr (sizeof(T) == 2) {
+                if (g.low) {
+                    WaRaw<T> rl = wa_zero<T>();
+                    if (mine && ch < g.D) rl = wa_load8<T>(lrow + ch);
+                    float fl[8];
+                    wa_floats<T>(rl, fl);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) fo[e] += fl[e];
+                }
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) dl = fmaf(fg[e], fo[e], dl);
             wa_pieces<T, PREC>(rg, gp[kb]);
@@ -919,7 +945,7 @@ int wa_dp(int D) { return D <= 32 ? 32 : D <= 64 ? 64 : 128; }
 WaArgs wa_args(const gfs3d_window_attn_args *a)
 {
     WaArgs g{};
-    g.q = a->q; g.k = a->k; g.v = a->v; g.out = a->out; g.dout = a->dout;
+    g.q = a->q; g.k = a->k; g.v = a->v; g.out = a->out; g.dout = a->dout; g.low = a->type == GFS3D_COMPUTE_F32 ? nullptr : a->out_low;
     g.qs = {a->q_stride[0], a->q_stride[1], a->q_stride[2]};
     g.ks = {a->k_stride[0], a->k_stride[1], a->k_stride[2]};
     g.vs = {a->v_stride[0], a->v_stride[1], a->v_stride[2]};
@@ -968,7 +994,7 @@ template <class T, int DP> bool wa_wide(const WaArgs &g)
 }
 template <class T, int DP, int NW> int wa_forward_queries(WaArgs g, void *out, hipStream_t st, const char *who)
 {
-    constexpr size_t im = 4ull * Mx<WaT<T>::PF>::NP * WaT<T>::KT * WaImg<DP>::ROWB, ou = (size_t)NW * WA_OUT<T, DP>, lds = im > ou ? im : ou;
+    constexpr size_t im = 4ull * Mx<WaT<T>::PF>::NP * (WA_KT<T, DP, NW>) * WaImg<DP>::ROWB, ou = (size_t)NW * WA_OUT<T, DP>, lds = im > ou ? im : ou;
     g.nblk = (int)(((long long)((g.N + 31) / 32) * g.HG + NW - 1) / NW);
     const size_t blocks = (size_t)g.B * g.G * g.nblk;
     GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);

@@ -160,7 +160,7 @@ class WindowAttnArgs(Structure):
         ("left", c_int), ("right", c_int), ("sinks", c_int), ("scale", c_float),
         ("q", c_void_p), ("k", c_void_p), ("v", c_void_p),
         ("q_stride", c_longlong * 3), ("k_stride", c_longlong * 3), ("v_stride", c_longlong * 3),
-        ("lengths", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+        ("lengths", c_void_p), ("out", c_void_p), ("out_low", c_void_p), ("lse", c_void_p),
         ("dout", c_void_p), ("dout_stride", c_longlong * 3),
         ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t),

@@ -1544,25 +1544,29 @@ class WindowAttentionFunction(torch.autograd.Function):
         out = torch.empty((a.B, a.N, a.H, a.D), dtype=q.dtype, device=q.device)
         grad = any(ctx.needs_input_grad[:3])
         lse = torch.empty((a.B, a.H, a.N), dtype=torch.float32, device=q.device) if grad else None
+        low = torch.empty_like(out) if grad and out.element_size() == 2 else None
         if out.numel():
             _window_inputs(a, q, k, v)
-            a.out, a.lse = out.data_ptr(), lse.data_ptr() if grad else None
+            a.out = out.data_ptr()
+            if grad:
+                a.lse, a.out_low = lse.data_ptr(), None if low is None else low.data_ptr()
             _launch("gfs3d_window_attn_forward", device, a)
         if grad:
-            ctx.save_for_backward(q, k, v, out, lse, lengths)
+            ctx.save_for_backward(q, k, v, out, low, lse, lengths)
             ctx.cfg = (left, right, sinks, scale)
         return out
 
     @staticmethod
     def backward(ctx, dout):
         _first_order("window_attention")
-        q, k, v, out, lse, lengths = ctx.saved_tensors
+        q, k, v, out, low, lse, lengths = ctx.saved_tensors
         a, _, device = _window_args("window_attention", q, k, v, *ctx.cfg, lengths)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
         if out.numel():
             dout = _heads4(dout)
             _window_inputs(a, q, k, v)
             a.out, a.lse, a.dout, a.dq, a.dk, a.dv = (t.data_ptr() for t in (out, lse, dout, dq, dk, dv))
+            a.out_low = None if low is None else low.data_ptr()
             a.dout_stride = dout.stride()[:3]
             nbytes = _lib.lib().gfs3d_window_attn_workspace_bytes(a.B, a.N, a.S, a.H, a.G, a.D, a.left, a.sinks, 0)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # from torch's allocator: a captured graph keeps its own

@@ -361,7 +361,9 @@ int gfs3d_attention_backward_mixed(const float *q, const float *k, const float *
  *   fp32 accuracy; bf16 and half products with fp32 scores, statistics and accumulators, gradients of half tensors on two bf16 pieces).
  *   lengths: (B) device int32 (clamped to 0..S), or NULL = S.  left / right at or above S: unlimited.  scale > 0.
  * forward (S == N): row i stands at position i.  lse (B, H, N) is written if not NULL: log2 of the sum of 2^(scaled scores
- *   log2 e), +inf for rows that see nothing (what the backward reads).
+ *   log2 e), +inf for rows that see nothing (what the backward reads).  out_low (out's shape and type), if not NULL and the type has 16
+ *   bits, receives what rounding took from out: with it the backward's dout . out is as exact as its products (without: the gradients
+ *   of q and k under a window of two keys are 3.7e-3 off for bf16, with it 2.5e-3; one rounding alone is 1.7e-3).
  * backward: dout -> dq, dk, dv; reads q, k, v, out, lse; deterministic (no atomics).
  * step: the N rows are the last positions of each sequence, row t at length - N + t; right is taken as 0 (S keys of capacity).
  * Workspace (device, 16-byte aligned): gfs3d_window_attn_workspace_bytes(..., step); 0 for the forward. */
@@ -373,6 +375,7 @@ typedef struct gfs3d_window_attn_args {
     long long q_stride[3], k_stride[3], v_stride[3];
     const int *lengths;
     void *out;
+    void *out_low;
     float *lse;
     const void *dout;
     long long dout_stride[3];
