@@ -793,7 +793,10 @@ __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4
             const int ch = 16 * kb + 8 * h;
             rk[kb] = wa_zero<T>();
             rv[kb] = wa_zero<T>();
-            if (r0 + j < len && ch < g.D) { rk[kb] = wa_load8<T>(kr + ch); rv[kb] = wa_load8<T>(vr + ch); }
+            if (r0 + j < len && (r0 + j >= first || r0 + j < g.sinks) && ch < g.D) {        // (what no row sees may be overwritten)
+                rk[kb] = wa_load8<T>(kr + ch);
+                rv[kb] = wa_load8<T>(vr + ch);
+            }
         }
     };
     const int step = NW * g.nchunk;

@@ -1589,7 +1589,8 @@ def window_attention(q, k, v, left: Optional[int] = None, right: Optional[int] =
 def window_attention_step(q, k, v, lengths, left: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:
     """window_attention (right = 0) for the last T rows of sequences whose keys and values are cached: q (B, T, H, D), k / v (B, S, G,
     D) with room for S rows, `lengths` (B,) the sequences' lengths with these T rows (a device tensor: no host read).  Row t stands at
-    position length - T + t; rows in front of the first position are zero.  No backward."""
+    position length - T + t; rows in front of the first position are zero.  Keys that none of the rows sees (behind the length, between
+    the sinks and the first row's window) are not read.  No backward."""
     _no_grad_form("window_attention_step", q, k, v)
     if lengths is None:
         raise RuntimeError("gfs3d.window_attention_step: lengths (B,) is needed")

@@ -166,11 +166,14 @@ STEP = [
 def test_window_attention_step(case, dtype):
     B, T, S, H, G, D, left, sinks, lens = STEP[case]
     q, k, v = rnd(31, (B, T, H, D), dtype), rnd(32, (B, S, G, D), dtype), rnd(33, (B, S, G, D), dtype)
-    for b, n in enumerate(lens):                              # what lies behind a sequence is not read
-        k[b, n:] = math.nan
-        v[b, n:] = math.inf
+    for b, n in enumerate(lens):                              # what lies behind a sequence, or between sinks and window, is not read
+        gone = max(sinks, n - T - left) if left is not None else 0
+        for a_, b_ in ((n, S), (sinks, gone)):
+            k[b, a_:b_] = math.nan
+            v[b, a_:b_] = math.inf
     lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
     out = ops().window_attention_step(q, k, v, lengths, left=left, sinks=sinks)
+    k, v = k.nan_to_num(0, 0, 0), v.nan_to_num(0, 0, 0)
     O.check(f"{dtype} {STEP[case]}", out, O.attention(q, k, v, left, 0, sinks, lens, step=True, dtype=dtype)["out"])
 
 
