@@ -5,7 +5,7 @@
  * The reference has no FFI: its "interface" for this path is the set of Python
  * functions below.  Each entry point names the reference
  * code it replaces.  All pointers are DEVICE pointers unless stated; all
- * tensors are dense fp32 in the layout given; `stream` is a hipStream_t passed
+ * tensors are dense fp32 in the layout given (K7 - K9: types and strides in their structs); `stream` is a hipStream_t passed
  * as void* (NULL = default stream).  No entry point allocates, frees or
  * synchronises: callers hand in outputs and a workspace (graph-capture safe).
  * The training EdgeConv forward forks a few kernels onto a library-owned side
