@@ -722,22 +722,26 @@ __global__ void __launch_bounds__(64 * (WA_SINK_NW<T, DP>), 1) wa_bwd_sink_kerne
         if (on) wa_dkv_tile<T, PREC, DP, 32, true>(g, Qimg, Gimg, Ls, Ds, p0, k0, len, lane, kp, vp, AK, AV);
         __syncthreads();
     }
-    float *sum = reinterpret_cast<float *>(at_smem);                                            // [dK | dV][channel][key]
-    for (int w = 0; w < NW; ++w) {
-        if (wv == w) {
+    float *sum = reinterpret_cast<float *>(at_smem);                                            // [wave][dK | dV][channel][key]
 #pragma unroll
-            for (int d = 0; d < ND; ++d)
+    for (int d = 0; d < ND; ++d)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float *a = sum + (32 * d + at_drow(r, h)) * 32 + j, *v = a + DP * 32;
-                    *a = w ? *a + AK[d][r] : AK[d][r];
-                    *v = w ? *v + AV[d][r] : AV[d][r];
-                }
+        for (int r = 0; r < 16; ++r) {
+            float *a = sum + (wv * 2 * DP + 32 * d + at_drow(r, h)) * 32 + j;
+            a[0] = AK[d][r];
+            a[DP * 32] = AV[d][r];
         }
-        __syncthreads();
-    }
+    __syncthreads();
     float *o = g.part + (size_t)blockIdx.x * (2 * DP * 32);
-    for (int e = t; e < 2 * DP * 32; e += 64 * NW) o[e] = sum[e];
+    for (int e = 4 * t; e < 2 * DP * 32; e += 256 * NW) {
+        float4 x = *reinterpret_cast<const float4 *>(sum + e);
+#pragma unroll
+        for (int w = 1; w < NW; ++w) {
+            const float4 y = *reinterpret_cast<const float4 *>(sum + w * 2 * DP * 32 + e);
+            x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+        }
+        *reinterpret_cast<float4 *>(o + e) = x;
+    }
 }
 
 // the chunks of a sink tile added, in order, into the first: thread = 4 values, grid (values / 1024, tiles)
@@ -898,30 +902,29 @@ __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4
     }
 }
 
-// joins the nchunk partial softmaxes of one (sequence, key head, 32 columns): thread = (column, 4 channels)
+// joins the nchunk partial softmaxes of one (sequence, key head, 32 columns): thread = (column, 4 channels), all of it at once
 template <class T, int DP>
-__global__ void __launch_bounds__(256) wa_join_kernel(const WaArgs g, T *__restrict__ out)
+__global__ void __launch_bounds__(8 * DP) wa_join_kernel(const WaArgs g, T *__restrict__ out)
 {
-    const int t = threadIdx.x, j = t & 31;
+    constexpr int PER = 64 + DP * 32;
+    const int t = threadIdx.x, j = t & 31, ch = 4 * (t >> 5);
     const int cb = blockIdx.x % g.nblk, bg = blockIdx.x / g.nblk, b = bg / g.G, gi = bg % g.G;
     const int col = cb * 32 + j, hs = col / g.N, head = gi * g.HG + hs, tq = col % g.N;
-    if (hs >= g.HG) return;
-    const float *pt = g.part + (size_t)blockIdx.x * g.nchunk * (64 + DP * 32);
-    float M = -__builtin_inff(), Lt = 0.f;
-    for (int s = 0; s < g.nchunk; ++s) M = fmaxf(M, pt[(size_t)s * (64 + DP * 32) + j]);
-    for (int ch = 4 * (t >> 5); ch < g.D; ch += 32) {
-        float o[4] = {0.f, 0.f, 0.f, 0.f};
-        Lt = 0.f;
-        for (int s = 0; s < g.nchunk; ++s) {
-            const float *p = pt + (size_t)s * (64 + DP * 32), ms = p[j];
-            const float f = ms == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ms - M);
-            Lt = fmaf(p[32 + j], f, Lt);
+    if (hs >= g.HG || ch >= g.D) return;
+    const float *pt = g.part + (size_t)blockIdx.x * g.nchunk * PER;
+    float M = -__builtin_inff(), Lt = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < g.nchunk; ++s) M = fmaxf(M, pt[(size_t)s * PER + j]);
+#pragma unroll 4
+    for (int s = 0; s < g.nchunk; ++s) {
+        const float *p = pt + (size_t)s * PER, ms = p[j];
+        const float f = ms == -__builtin_inff() ? 1.f : __builtin_amdgcn_exp2f(ms - M);
+        Lt = fmaf(p[32 + j], f, Lt);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(p[64 + (ch + e) * 32 + j], f, o[e]);
-        }
-        const float inv = Lt > 0.f ? 1.f / Lt : (Lt != Lt ? Lt : 0.f);
-        wa_store4<T>(out + (((size_t)b * g.N + tq) * g.H + head) * g.D + ch, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(p[64 + (ch + e) * 32 + j], f, o[e]);
     }
+    const float inv = Lt > 0.f ? 1.f / Lt : (Lt != Lt ? Lt : 0.f);
+    wa_store4<T>(out + (((size_t)b * g.N + tq) * g.H + head) * g.D + ch, o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1051,7 +1054,7 @@ template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *d
     if (int rc = wa_backward_queries<T, DP>(g, dq, st, who)) return rc;
     if (g.nst > 0) {
         constexpr int NW = (WA_SINK_NW<T, DP>);
-        constexpr size_t ws = (size_t)NW * (2 * img + 256), sum = 2ull * DP * 32 * sizeof(float), lsk = ws > sum ? ws : sum;
+        constexpr size_t ws = (size_t)NW * (2 * img + 256), sum = 2ull * NW * DP * 32 * sizeof(float), lsk = ws > sum ? ws : sum;
         const size_t blocks = (size_t)g.B * g.G * g.nst * g.nchunk;
         GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
         GFS3D_ENSURE_LDS((wa_bwd_sink_kernel<T, DP>), lsk, who);
@@ -1077,7 +1080,7 @@ template <class T, int DP, bool WIDE> int wa_step_go(const WaArgs &g, void *out,
     hipLaunchKernelGGL((wa_step_kernel<T, DP, WIDE>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)out);
     GFS3D_LAUNCH_CHECK("wa_step_kernel");
     if (g.nchunk > 1) {
-        hipLaunchKernelGGL((wa_join_kernel<T, DP>), dim3((unsigned)groups), dim3(256), 0, st, g, (T *)out);
+        hipLaunchKernelGGL((wa_join_kernel<T, DP>), dim3((unsigned)groups), dim3(8 * DP), 0, st, g, (T *)out);
         GFS3D_LAUNCH_CHECK("wa_join_kernel");
     }
     return GFS3D_OK;
