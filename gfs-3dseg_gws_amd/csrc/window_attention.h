@@ -155,6 +155,7 @@ template <class T, int DP, int R, int NT> struct WaStage {
 #pragma unroll
             for (int n = 0; n < NCH; ++n) r[n] = *reinterpret_cast<const WaRaw<T> *>(p + off[n]);
         } else {
+            asm volatile("");                         // or the compiler folds both branches into masked loads
 #pragma unroll
             for (int n = 0; n < NCH; ++n) {
                 const int c = t + n * NT;
@@ -762,9 +763,11 @@ template <int DP> __global__ void __launch_bounds__(256) wa_sink_sum_kernel(floa
 // Columns of a wave's tile = up to 32 (head of the key head, row) pairs, so that a cached key is read once for all of them.  The
 // visible key tiles of a sequence are dealt to the waves of its nchunk workgroups in turn; each wave keeps its own running
 // softmax, the waves of a workgroup join through LDS, the workgroups (nchunk > 1) through part[..][m | l | O] and a second kernel.
-// HBM-bound: a wave has two tiles of K and V in flight (32 keys x 128 channels: 32 KB).  WIDE: up to 16 waves of one workgroup share
-// short caches, which saves the second launch; otherwise 4, so that workgroups at different stages share a CU.
-template <class T, int DP, bool WIDE> constexpr int WA_STEP_NW = !WIDE ? 4 : sizeof(T) == 4 ? (DP == 128 ? 4 : 8) : 8;
+// HBM-bound: a wave has a tile of K and V in flight (32 keys x 128 channels: 16 KB) beside the one it computes.  64 sequences x 4112 keys
+// x 4 key heads x 128 bf16: 122 us, 4.4 TB/s; with lane masks around the loads of every tile 148.  WIDE: eight waves of one workgroup
+// share short caches, which saves the second launch (1028 keys x 64: 12.2 us for 15.2); otherwise 4, so that workgroups at
+// different stages share a CU.
+template <class T, int DP, bool WIDE> constexpr int WA_STEP_NW = WIDE && !(sizeof(T) == 4 && DP == 128) ? 8 : 4;
 template <class T, int DP, bool WIDE>
 __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4 && DP == 128 ? 1 : 2) wa_step_kernel(const WaArgs g, T *__restrict__ out)
 {
@@ -795,14 +798,24 @@ __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4
     auto load = [&](int tt) {
         const int r0 = row0(tt);
         const T *kr = kb_ + (long long)(r0 + j) * g.ks.r, *vr = vb + (long long)(r0 + j) * g.vs.r;
+        if (r0 >= first && r0 + 32 <= len && g.D == DP) {                  // (masked loads of every tile: 148 us for 122, see above)
 #pragma unroll
-        for (int kb = 0; kb < NK; ++kb) {
-            const int ch = 16 * kb + 8 * h;
-            rk[kb] = wa_zero<T>();
-            rv[kb] = wa_zero<T>();
-            if (r0 + j < len && (r0 + j >= first || r0 + j < g.sinks) && ch < g.D) {        // (what no row sees may be overwritten)
-                rk[kb] = wa_load8<T>(kr + ch);
-                rv[kb] = wa_load8<T>(vr + ch);
+            for (int kb = 0; kb < NK; ++kb) {
+                rk[kb] = wa_load8<T>(kr + 16 * kb + 8 * h);
+                rv[kb] = wa_load8<T>(vr + 16 * kb + 8 * h);
+            }
+        } else {
+            asm volatile("");
+            const bool seen = r0 + j < len && (r0 + j >= first || r0 + j < g.sinks);        // what no row sees may be overwritten
+#pragma unroll
+            for (int kb = 0; kb < NK; ++kb) {
+                const int ch = 16 * kb + 8 * h;
+                rk[kb] = wa_zero<T>();
+                rv[kb] = wa_zero<T>();
+                if (seen && ch < g.D) {
+                    rk[kb] = wa_load8<T>(kr + ch);
+                    rv[kb] = wa_load8<T>(vr + ch);
+                }
             }
         }
     };
@@ -983,8 +996,8 @@ void wa_dkv_plan(WaArgs &g, bool most = false)       // most: the bound over all
 }
 size_t wa_split_floats(const WaArgs &g) { return g.nsplit > 1 ? (size_t)g.nsplit * 2 * g.B * g.N * g.G * g.D : 0; }
 size_t wa_sink_floats(const WaArgs &g) { return (size_t)g.B * g.G * g.nst * g.nchunk * 2 * wa_dp(g.D) * 32; }
-// Short caches, or as many sequences as CUs twice over: one workgroup each (wide, no second launch); else the keys are split until there
-// are four workgroups to a CU, four tiles to a wave at least
+// Short caches (at most 64 tiles): one workgroup of eight waves each and no second launch; else the keys are split until there are four
+// workgroups to a CU (64 x 4112 keys x 4 heads x 128: 122 us; two 155 with masked loads for 148, eight 128), four tiles to a wave at least
 void wa_step_plan(WaArgs &g, bool &wide)
 {
     g.nblk = (int)(((long long)g.HG * g.N + 31) / 32);
