@@ -7,17 +7,18 @@
 // Part of attention.hip (the operand images and the transposed LDS read are those of K5 there).
 //
 // Forward: a wave owns one unit = 32 queries of one head (the QUERY on the lane, S^T = K Q^T, so that a query's running maximum,
-// sum and accumulators are in-lane), the four waves of a workgroup own consecutive units with the heads of one key head innermost:
-// they share every staged key tile.  Tiles outside all four windows are never staged, tiles outside a wave's own window cost it
+// sum and accumulators are in-lane), the four or eight waves of a workgroup own consecutive units with the heads of one key head innermost:
+// they share every staged key tile.  Tiles outside all of their windows are never staged, tiles outside a wave's own window cost it
 // nothing but the barrier, and only tiles that a window edge, the diagonal or the length cuts pay for the element mask.
 // Backward: dQ with the query on the lane (it also leaves delta_i = dout_i . o_i), dK / dV with the key on the lane, looping over the
 // heads of the key head; what the sinks receive from queries beyond their window (all rows of a long sequence) is summed by
-// its own kernel in row chunks, and the chunks are joined, in order, where dK / dV of those keys are written.  No atomics.
+// its own kernel in row chunks, the chunks are added in order by another, and their sum joins where dK / dV of those keys are
+// written.  No atomics.
 // Scores, softmax statistics, accumulators and all sums over heads or chunks are fp32.  Probabilities and dS are rounded to the operand
 // type of the matrix cores: bf16 / half for those tensors, exact 3-way bf16 splits (PREC_X6) for fp32; the gradients of half
 // tensors take two bf16 pieces (PREC_X3), whose range is fp32's - a mean loss underflows in half.
-// Measured (2 x 65536 rows, 8 heads x 64, bf16, 512 to either side + 16 sinks): forward 420 us (0.67 PFLOP/s of visible pairs), dQ 575
-// (0.73), dK / dV 780 (0.72), sinks 78.  Bound by vector issue: of a forward tile's cycles the vector pipe is busy 64 %, the matrix
+// Measured (2 x 65536 rows, 8 heads x 64, bf16, 512 to either side + 16 sinks): forward 420 us (0.67 PFLOP/s of visible pairs), dQ 580
+// (0.72), dK / dV 780 (0.72), sinks 75.  Bound by vector issue: of a forward tile's cycles the vector pipe is busy 64 %, the matrix
 // pipe 32 %, and four waves per SIMD (128 registers) did better than every form that overlaps the two within a wave at two.
 
 namespace gfs3d {
@@ -42,7 +43,8 @@ template <class T> struct WaT;
 template <> struct WaT<float> { static constexpr int PF = PREC_X6, PB = PREC_X6; };
 template <> struct WaT<__bf16> { static constexpr int PF = PREC_BF16, PB = PREC_BF16; };
 template <> struct WaT<_Float16> { static constexpr int PF = PREC_F16, PB = PREC_X3; };
-// keys of a staged tile in the forward
+// keys of a staged tile in the forward (eight waves, 128 channels: causal 8192 x 16 heads half 655 us with 128 keys, 672 with 64; 64
+// channels: no difference)
 template <class T, int DP, int NW> constexpr int WA_KT = sizeof(T) == 4 ? 32 : NW == 8 && DP == 128 ? 128 : 64;
 
 // eight consecutive channels as they lie in memory
@@ -155,7 +157,6 @@ template <class T, int DP, int R, int NT> struct WaStage {
 #pragma unroll
             for (int n = 0; n < NCH; ++n) r[n] = *reinterpret_cast<const WaRaw<T> *>(p + off[n]);
         } else {
-            asm volatile("");                         // or the compiler folds both branches into masked loads
 #pragma unroll
             for (int n = 0; n < NCH; ++n) {
                 const int c = t + n * NT;
@@ -241,38 +242,31 @@ template <bool FAR, class X> __device__ __forceinline__ void wa_mask(int j0, int
 }
 
 // ------------------------------------------------------------------ forward
-// NS 32-key subtiles of the staged tile, from Kc / Vc on (keys j0 ..): scores, running softmax, products.  `whole`: every key is seen
-template <class T, int DP, int KT, int NS>
+// 32 keys of the staged tile, from Kc / Vc on (keys j0 ..): scores, running softmax, products.  `whole`: every key is seen.  The
+// running maximum follows only when a row's has grown by WA_LAZY (in base 2): most tiles then leave the accumulators alone
+template <class T, int DP, int KT>
 __device__ __forceinline__ void wa_fwd_tile(const unsigned char *Kc, const unsigned char *Vc, int j0, int lane, float c, float thr, bool whole,
                                             int lo, int hi, int far, const uint4 (&qp)[DP / 16][Mx<WaT<T>::PF>::NP], float &m, float &mc,
                                             float &l, f32x16 (&O)[DP / 32])
 {
-    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, ROWB = WaImg<DP>::ROWB, ND = DP / 32;
+    constexpr int PREC = WaT<T>::PF, NP = Mx<PREC>::NP, ND = DP / 32;
     const int j = lane & 31, h = lane >> 5;
-    f32x16 acc[NS];
+    f32x16 acc;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[s][r] = 0.f;
-#pragma unroll
-        for (int kb = 0; kb < DP / 16; ++kb) {
-            uint4 ak[NP];
-            wa_rowfrag<PREC, DP, KT>(Kc, 32 * s + j, h, kb, ak);
-            mm_mac<PREC>(ak, qp[kb], acc[s]);
-        }
+    for (int kb = 0; kb < DP / 16; ++kb) {
+        uint4 ak[NP];
+        wa_rowfrag<PREC, DP, KT>(Kc, j, h, kb, ak);
+        mm_mac<PREC>(ak, qp[kb], acc);
     }
     if (!whole) {
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            if (j0 + 32 * s >= far) wa_mask<false>(j0 + 32 * s, h, lo, hi, 0, -__builtin_inff(), acc[s]);
-            else wa_mask<true>(j0 + 32 * s, h, lo, hi, min(far, hi + 1), -__builtin_inff(), acc[s]);
-        }
+        if (j0 >= far) wa_mask<false>(j0, h, lo, hi, 0, -__builtin_inff(), acc);
+        else wa_mask<true>(j0, h, lo, hi, min(far, hi + 1), -__builtin_inff(), acc);
     }
-    float tmax = acc[0][0];
+    float tmax = acc[0];
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, acc[s][r]);
+    for (int r = 0; r < 16; ++r) tmax = fmaxf(tmax, acc[r]);
     tmax = wa_max32(tmax);
     if (__ballot(tmax > m + thr) != 0ull) {
         const float m_new = fmaxf(m, tmax), mc_new = m_new == -__builtin_inff() ? 0.f : m_new * c;
@@ -285,23 +279,20 @@ __device__ __forceinline__ void wa_fwd_tile(const unsigned char *Kc, const unsig
 #pragma unroll
             for (int r = 0; r < 16; ++r) O[d][r] *= sc;
     }
+    float pd[16];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-        float pd[16];
+    for (int r = 0; r < 16; ++r) {
+        pd[r] = __builtin_amdgcn_exp2f(fmaf(acc[r], c, -mc));
+        l += pd[r];
+    }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            pd[r] = __builtin_amdgcn_exp2f(fmaf(acc[s][r], c, -mc));
-            l += pd[r];
-        }
+    for (int ks = 0; ks < 2; ++ks) {
+        uint4 pp[NP], av[NP];
+        at_regfrag<PREC>(pd, ks, pp);
 #pragma unroll
-        for (int ks = 0; ks < 2; ++ks) {
-            uint4 pp[NP], av[NP];
-            at_regfrag<PREC>(pd, ks, pp);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) {
-                wa_trfrag<PREC, DP, KT>(Vc + 32 * s * ROWB, lane, d, ks, av);
-                mm_mac<PREC>(av, pp, O[d]);
-            }
+        for (int d = 0; d < ND; ++d) {
+            wa_trfrag<PREC, DP, KT>(Vc, lane, d, ks, av);
+            mm_mac<PREC>(av, pp, O[d]);
         }
     }
 }
@@ -363,7 +354,7 @@ __global__ void __launch_bounds__(64 * NW, DP == 128 ? (sizeof(T) == 4 ? 1 : 2) 
 #pragma unroll
             for (int s = 0; s < 32 * SUB; s += 32)
                 if (holds(j0 + s))
-                    wa_fwd_tile<T, DP, KT, 1>(Kc + s * ROWB, Vc + s * ROWB, j0 + s, lane, g.c, thr, whole(j0 + s, 32), lo, hi, far, qp, m, mc, l, O);
+                    wa_fwd_tile<T, DP, KT>(Kc + s * ROWB, Vc + s * ROWB, j0 + s, lane, g.c, thr, whole(j0 + s, 32), lo, hi, far, qp, m, mc, l, O);
         }
         if (tt + 1 < nt) { sk.template put<PREC>(Kimg + (cur ^ 1) * IMG, t); sv.template put<PREC>(Vimg + (cur ^ 1) * IMG, t); }
         __syncthreads();
@@ -953,6 +944,8 @@ int wa_check(const char *who, const gfs3d_window_attn_args *a)
     GFS3D_REQUIRE(a->scale > 0.f && a->scale < 3e38f, "%s: scale %g must be positive and finite", who, (double)a->scale);
     GFS3D_REQUIRE(a->q && a->k && a->v && a->out, "%s: NULL buffer", who);
     const int gran = 16 / (a->type == GFS3D_COMPUTE_F32 ? 4 : 2);
+    const void *written[6] = {a->out, a->out_low, a->dq, a->dk, a->dv, a->workspace};
+    for (const void *w : written) GFS3D_REQUIRE(((uintptr_t)w & 15) == 0, "%s: an output or the workspace is not aligned to 16 bytes", who);
     const long long *st[4] = {a->q_stride, a->k_stride, a->v_stride, a->dout_stride};
     const void *pt[4] = {a->q, a->k, a->v, a->dout};
     for (int n = 0; n < 4; ++n) {

@@ -30,7 +30,7 @@ def _window(m, **kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(type=5), b"type"), (dict(N=0, S=0), b"bad shape"), (dict(H=3, G=2), b"key heads"), (dict(D=60), b"head size"), (dict(D=136), b"head size"),
     (dict(left=-1), b"left"), (dict(sinks=-2), b"sinks"), (dict(scale=0.0), b"scale"), (dict(scale=float("nan")), b"scale"),
-    (dict(scale=float("inf")), b"scale"), (dict(q=None), b"NULL"), (dict(k=4100), b"16 bytes"), (dict(S=63), b"differs"),
+    (dict(scale=float("inf")), b"scale"), (dict(q=None), b"NULL"), (dict(k=4100), b"16 bytes"), (dict(out=4104), b"16 bytes"), (dict(S=63), b"differs"),
     (dict(v_stride=(ctypes.c_longlong * 3)(8192, 100, 64)), b"stride"), (dict(q_stride=(ctypes.c_longlong * 3)(8192, -128, 64)), b"stride"),
 ])
 def test_window_attention_refuses(kw, text):
