@@ -60,7 +60,7 @@ def attention(q, k, v, left, right, sinks, lengths, scale=None, step=False, dout
     g = clean(dout.detach().cpu().double(), krow)
     prod = 2.0 ** -15 if dtype == torch.float16 else U32 * 8
     wg = {torch.float32: U32 * 4, torch.bfloat16: u(torch.bfloat16), torch.float16: 2.0 ** -15}[dtype]
-    eg = es + 2 * prod * smax + (2 * uo * 0 if dtype == torch.float32 else 0)
+    eg = es + 2 * prod * smax
     delta = (g * o).sum(-1).permute(0, 2, 1)[..., None]
     derr = (g.abs() * (got["out"][1] + (D + 8) * U32 * o.abs())).sum(-1).permute(0, 2, 1)[..., None]
     dp = mm("bihd,bjhd->bhij", g, v)

@@ -547,3 +547,26 @@ def test_two_captured_steps_share_nothing():
         torch.cuda.synchronize()
         for i in range(2):
             assert torch.equal(outs[i], want[i]) and torch.equal(again[i], want[i])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_large_batches_equal_their_parts(D, dtype):
+    """A batch large enough for eight-wave workgroups and unsplit key gradients, against two of its sequences alone (four waves, rows of
+    dK and dV split): the forward takes the same key tiles in the same order, so it is equal; the sums of the gradients differ in order."""
+    o = ops()
+    B, N, H, G = 130, 515, 8, 4
+    lens = torch.tensor([515 - 7 * (b % 30) for b in range(B)], dtype=torch.int32, device="cuda")
+    q, k, v, g = (rnd(140 + n, (B, N, h, D), dtype) for n, h in enumerate((H, G, G, H)))
+    for left, right, sinks in ((70, 33, 5), (None, 0, 0)):
+        whole = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = o.window_attention(*whole, left=left, right=right, sinks=sinks, lengths=lens)
+        grads = torch.autograd.grad(out, whole, g)
+        for b in (0, 31, 128):
+            part = [t[b:b + 2].clone().requires_grad_() for t in (q, k, v)]
+            one = o.window_attention(*part, left=left, right=right, sinks=sinks, lengths=lens[b:b + 2])
+            assert torch.equal(one, out[b:b + 2])
+            want = O.attention(q[b:b + 2], k[b:b + 2], v[b:b + 2], left, right, sinks, lens[b:b + 2].tolist(), dout=g[b:b + 2], dtype=dtype)
+            for name, x, y in zip(("dq", "dk", "dv"), torch.autograd.grad(one, part, g[b:b + 2]), grads):
+                O.check(f"{name} alone", x, want[name])
+                O.check(f"{name} of the batch", y[b:b + 2], want[name])
