@@ -12,6 +12,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from . import _lib
 from ._lib import PointwiseArgs, PointwiseBwdArgs, PW_MAX_LAYERS, PW_MAX_SEGS, PW_SEG_WIDTH, EdgeConvArgs, EdgeConvBwdArgs
@@ -1469,7 +1470,14 @@ def _need_typed(who: str, first: torch.Tensor, *rest: torch.Tensor) -> int:
     return first.get_device()
 
 
+def _no_tangents(who: str, *tensors) -> None:
+    """Forward-mode derivatives are refused, not dropped: a tensor that carries a tangent need not require a gradient."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"gfs3d.{who} has no forward-mode derivative: an input carries a tangent (torch.autograd.forward_ad)")
+
+
 def _no_grad_form(who: str, *tensors) -> None:
+    _no_tangents(who, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"gfs3d.{who} has no backward: call it under torch.no_grad() or on detached tensors")
 
@@ -1708,6 +1716,7 @@ def rotary(q, k, positions, freqs, magnitude: float = 1.0, layout: str = "half")
     P = freqs.shape[0] * axes
     if P < 1 or 2 * P > D or P > 1024 or H < 1 or (k is not None and k.shape[2] < 1):
         raise RuntimeError(f"gfs3d.rotary: {axes} axes of {freqs.shape[0]} pairs do not fit heads of {D} channels")
+    _no_tangents("rotary", q, k, positions, freqs)
     positions, freqs = positions.contiguous(), freqs.contiguous()
     interleaved = 1 if layout == "interleaved" else 0
     if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
@@ -1804,6 +1813,7 @@ def rms_norm(x, weight, eps: float = 1e-6, residual: Optional[torch.Tensor] = No
     s = x + residual rounded to the residual's type (the residual stream; float32 beside 16-bit x is allowed), which is returned
     too: (y, s).  The statistics are those of s as it is stored, in fp32.  weight (C,) float32 or x's type; C up to 16384.
     Differentiable once in x, weight and residual, deterministic."""
+    _no_tangents("rms_norm", x, weight, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
         return RmsNormFunction.apply(x, weight, residual, float(eps))
     y, _, stream, _, _ = _rms_forward("rms_norm", x, weight, eps, residual)
