@@ -1482,8 +1482,9 @@ def _no_grad_form(who: str, *tensors) -> None:
         raise RuntimeError(f"gfs3d.{who} has no backward: call it under torch.no_grad() or on detached tensors")
 
 
-def _first_order(who: str) -> None:
-    """In a backward: gradients of gradients (create_graph=True) are refused, not left out."""
+def _first_order(who: str, *grads) -> None:
+    """In a backward: gradients of gradients (create_graph=True, or forward mode through the backward) are refused, not left out."""
+    _no_tangents(f"{who}'s backward", *grads)
     if torch.is_grad_enabled():
         raise RuntimeError(f"gfs3d.{who}: the backward is not differentiable (create_graph=True)")
 
@@ -1566,7 +1567,7 @@ class WindowAttentionFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        _first_order("window_attention")
+        _first_order("window_attention", dout)
         q, k, v, out, low, lse, lengths = ctx.saved_tensors
         a, _, device = _window_args("window_attention", q, k, v, *ctx.cfg, lengths)
         dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
@@ -1680,7 +1681,7 @@ class RotaryFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dq, dk):
-        _first_order("rotary")
+        _first_order("rotary", dq, dk)
         positions, freqs = ctx.saved_tensors
         if dq is None and dk is None:
             return (None,) * 7
@@ -1779,7 +1780,7 @@ class RmsNormFunction(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy, ds=None):
-        _first_order("rms_norm")
+        _first_order("rms_norm", dy, ds)
         s, weight, rstd = ctx.saved_tensors
         dtype, eps, has_res = ctx.cfg
         if dy is None and ds is None:

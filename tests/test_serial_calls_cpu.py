@@ -43,3 +43,21 @@ def test_forward_mode_tangents_are_refused(ops, who, name, grad):
         del ops.calls[:]
         with pytest.raises((RuntimeError, NotImplementedError)):
             CALLS[who][1](ops, t)
+
+
+@pytest.mark.parametrize("who", ["rotary", "rms_norm", "window_attention"])
+def test_forward_mode_tangents_of_gradients_are_refused(ops, who):
+    """Forward over reverse: a gradient that carries a tangent enters no backward that would drop it."""
+    names, call = CALLS[who]
+    t = _inputs(ops)
+    t = {n: x.requires_grad_() if n in ("q", "k", "v", "x", "weight", "residual") else x for n, x in t.items()}
+    ins = [t[n] for n in names if t[n].requires_grad]
+    with forward_ad.dual_level():
+        outs = call(ops, t)
+        outs = outs if isinstance(outs, tuple) else (outs,)
+        plain = [torch.ones_like(o) for o in outs]
+        torch.autograd.grad(outs, ins, plain, retain_graph=True)
+        for n in range(len(outs)):
+            duals = [forward_ad.make_dual(g, torch.ones_like(g)) if m == n else g for m, g in enumerate(plain)]
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad(outs, ins, duals, retain_graph=True)
