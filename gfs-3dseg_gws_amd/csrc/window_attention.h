@@ -971,12 +971,15 @@ WaArgs wa_args(const gfs3d_window_attn_args *a)
     g.scale = a->scale; g.c = a->scale * 1.4426950408889634f;
     return g;
 }
-// the sinks' gradient kernel runs where some row lies beyond the first key's window; at most 32 chunks of at least 8 row tiles
+// the sinks' gradient kernel runs where some row lies beyond the first key's window; at most 32 chunks of at least 8 row tiles, and
+// only until every CU has four workgroups: each chunk leaves fp32 sums of its 32 keys, which otherwise outgrow the tensors
 void wa_sink_plan(WaArgs &g)
 {
     g.nst = g.sinks > 0 && g.N > g.left + 1 ? (g.sinks + 31) / 32 : 0;
-    const long long tiles = (long long)((g.N + 31) / 32) * g.HG;
-    g.nchunk = (int)(tiles / 8 < 1 ? 1 : tiles / 8 > 32 ? 32 : tiles / 8);
+    const long long tiles = (long long)((g.N + 31) / 32) * g.HG, keys = (long long)g.B * g.G * g.nst;
+    long long n = tiles / 8 > 32 ? 32 : tiles / 8;
+    if (keys > 0 && n > (1023 + keys) / keys) n = (1023 + keys) / keys;
+    g.nchunk = (int)(n < 1 ? 1 : n);
 }
 // dK, dV: workgroups of 128 keys, their turns split until every CU has two workgroups (at most 8 ways, 4 turns at least)
 void wa_dkv_plan(WaArgs &g, bool most = false)       // most: the bound over all types and reaches
@@ -1066,10 +1069,8 @@ template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *d
         GFS3D_ENSURE_LDS((wa_bwd_sink_kernel<T, DP>), lsk, who);
         hipLaunchKernelGGL((wa_bwd_sink_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lsk, st, g);
         GFS3D_LAUNCH_CHECK("wa_bwd_sink_kernel");
-        if (g.nchunk > 1) {
-            const size_t tiles = (size_t)g.B * g.G * g.nst;
-            GFS3D_REQUIRE(tiles < 65536, "%s: %zu sink tiles", who, tiles);
-            hipLaunchKernelGGL((wa_sink_sum_kernel<DP>), dim3(2 * DP * 32 / 1024, (unsigned)tiles), dim3(256), 0, st, g.part, g.nchunk);
+        if (g.nchunk > 1) {                                  // (then there are fewer than 1024 tiles)
+            hipLaunchKernelGGL((wa_sink_sum_kernel<DP>), dim3(2 * DP * 32 / 1024, (unsigned)(g.B * g.G * g.nst)), dim3(256), 0, st, g.part, g.nchunk);
             GFS3D_LAUNCH_CHECK("wa_sink_sum_kernel");
         }
     }

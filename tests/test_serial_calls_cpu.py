@@ -61,3 +61,24 @@ def test_forward_mode_tangents_of_gradients_are_refused(ops, who):
             duals = [forward_ad.make_dual(g, torch.ones_like(g)) if m == n else g for m, g in enumerate(plain)]
             with pytest.raises(RuntimeError):
                 torch.autograd.grad(outs, ins, duals, retain_graph=True)
+
+
+def _lib():
+    import __graft_entry__  # noqa: F401  (torch first: maps the HIP runtime the library binds to)
+    from gfs3d import _lib as m
+    return m.lib()
+
+
+@pytest.mark.parametrize("B,N,H,G,D,left,sinks", [
+    (64, 8192, 32, 8, 128, 1024, 512), (2, 65536, 8, 8, 64, 512, 16384), (8192, 512, 8, 8, 8, 8, 4), (2, 65536, 8, 8, 64, 512, 16),
+    (32, 2048, 1, 1, 64, 128, 4), (1, 8192, 64, 1, 128, 0, 32), (3, 100000, 6, 2, 40, 100, 1000), (1, 33, 1, 1, 32, 0, 33)])
+def test_the_backward_s_workspace_is_bounded_by_its_tensors(B, N, H, G, D, left, sinks):
+    """delta; the fp32 sums of the sink keys' dK and dV in whole tiles of 32, in several chunks of rows only while there are fewer than
+    2048 of them; and up to eight fp32 dK and dV where fewer than 512 workgroups of 128 keys exist."""
+    dp = 32 if D <= 32 else 64 if D <= 64 else 128
+    tiles = B * G * ((sinks + 31) // 32)
+    floats = B * H * N + 64 + max(tiles, 2048) * 2 * dp * 32
+    if B * G * ((N + 127) // 128) < 512:
+        floats += 8 * 2 * B * N * G * D
+    need = _lib().gfs3d_window_attn_workspace_bytes(B, N, N, H, G, D, left, sinks, 0)
+    assert 4 * B * H * N < need <= 4 * floats, (need, 4 * floats)
