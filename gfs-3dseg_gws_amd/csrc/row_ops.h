@@ -516,7 +516,7 @@ extern "C" int gfs3d_rotary(const gfs3d_rotary_args *a, void *stream)
     const long long want = (g.tokens + 1023) / 1024;
     g.tb = (int)(want < 1 ? 1 : want > most ? most : want);
     const long long blocks = (g.tokens + g.tb - 1) / g.tb;
-    GFS3D_REQUIRE(blocks < (1ll << 31) && (long long)g.tb * (g.heads[0] + g.heads[1]) * a->D < (1ll << 31), "%s: too many values", who);
+    GFS3D_REQUIRE(blocks * 256 < (1ll << 32) && (long long)g.tb * (g.heads[0] + g.heads[1]) * a->D < (1ll << 31), "%s: too many values", who);
     const int V = al ? vec : 1, W = V > 1 ? V : 2, heads = g.heads[0] + g.heads[1];
     g.per = g.interleaved ? (a->D + W - 1) / W : AP / V + (a->D - 2 * AP + V - 1) / V;
     const long long units = (long long)g.tb * heads * g.per;             // u < 2^32 / d: the product with the rounded-up reciprocal is exact

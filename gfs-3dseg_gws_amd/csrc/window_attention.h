@@ -1010,12 +1010,16 @@ template <class T, int DP> bool wa_wide(const WaArgs &g)
 {
     return sizeof(T) == 2 && (long long)g.B * g.G * (((g.N + 31) / 32 * (long long)g.HG + 7) / 8) >= 1024;
 }
+// a launch holds fewer than 2^32 threads
+#define WA_REQUIRE_GRID(blocks, threads, who) GFS3D_REQUIRE((size_t)(blocks) * (threads) < (1ull << 32), "%s: %zu workgroups", who, (size_t)(blocks))
+// workgroups of NW waves per (sequence, key head): a wave takes 32 rows of one head
+size_t wa_query_blocks(const WaArgs &g, int NW) { return ((size_t)((g.N + 31) / 32) * g.HG + NW - 1) / NW; }
 template <class T, int DP, int NW> int wa_forward_queries(WaArgs g, void *out, hipStream_t st, const char *who)
 {
     constexpr size_t im = 4ull * Mx<WaT<T>::PF>::NP * (WA_KT<T, DP, NW>) * WaImg<DP>::ROWB, ou = (size_t)NW * WA_OUT<T, DP>, lds = im > ou ? im : ou;
-    g.nblk = (int)(((long long)((g.N + 31) / 32) * g.HG + NW - 1) / NW);
-    const size_t blocks = (size_t)g.B * g.G * g.nblk;
-    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
+    const size_t blocks = (size_t)g.B * g.G * wa_query_blocks(g, NW);
+    WA_REQUIRE_GRID(blocks, 64 * NW, who);
+    g.nblk = (int)wa_query_blocks(g, NW);
     GFS3D_ENSURE_LDS((wa_fwd_kernel<T, DP, NW>), lds, who);
     hipLaunchKernelGGL((wa_fwd_kernel<T, DP, NW>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)out);
     GFS3D_LAUNCH_CHECK("wa_fwd_kernel");
@@ -1032,9 +1036,8 @@ template <class T, int DP> int wa_backward_queries(WaArgs g, void *dq, hipStream
 {
     constexpr int NW = 4;
     constexpr size_t im = 4ull * Mx<WaT<T>::PB>::NP * 32 * WaImg<DP>::ROWB, ou = (size_t)NW * WA_OUT<T, DP>, lds = im > ou ? im : ou;
-    g.nblk = (int)(((long long)((g.N + 31) / 32) * g.HG + NW - 1) / NW);
+    g.nblk = (int)wa_query_blocks(g, NW);
     const size_t blocks = (size_t)g.B * g.G * g.nblk;
-    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
     GFS3D_ENSURE_LDS((wa_bwd_dq_kernel<T, DP>), lds, who);
     hipLaunchKernelGGL((wa_bwd_dq_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)dq);
     GFS3D_LAUNCH_CHECK("wa_bwd_dq_kernel");
@@ -1046,7 +1049,6 @@ template <class T, int DP> int wa_backward_keys(WaArgs g, void *dk, void *dv, hi
     constexpr size_t im = 4 * ((size_t)Mx<WaT<T>::PB>::NP * QT * WaImg<DP>::ROWB + QT * sizeof(float)), ou = 4ull * WA_OUT<float, DP>, lds = im > ou ? im : ou;
     g.nblk = (g.N + 127) / 128;
     const size_t blocks = (size_t)g.nblk * g.B * g.G * g.nsplit;
-    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
     GFS3D_ENSURE_LDS((wa_bwd_dkv_kernel<T, DP>), lds, who);
     hipLaunchKernelGGL((wa_bwd_dkv_kernel<T, DP>), dim3((unsigned)blocks), dim3(256), lds, st, g, (T *)dk, (T *)dv);
     GFS3D_LAUNCH_CHECK("wa_bwd_dkv_kernel");
@@ -1060,14 +1062,16 @@ template <class T, int DP> int wa_backward_keys(WaArgs g, void *dk, void *dv, hi
 template <class T, int DP> int wa_backward(WaArgs g, void *dq, void *dk, void *dv, hipStream_t st, const char *who)
 {
     constexpr size_t img = (size_t)Mx<WaT<T>::PB>::NP * 32 * WaImg<DP>::ROWB;
+    const size_t pairs = (size_t)g.B * g.G, sinks = pairs * g.nst * g.nchunk;
+    WA_REQUIRE_GRID(pairs * wa_query_blocks(g, 4), 256, who);                // all refusals before the first launch
+    WA_REQUIRE_GRID(sinks, 64 * (WA_SINK_NW<T, DP>), who);
+    WA_REQUIRE_GRID(pairs * ((g.N + 127) / 128) * g.nsplit, 256, who);
     if (int rc = wa_backward_queries<T, DP>(g, dq, st, who)) return rc;
     if (g.nst > 0) {
         constexpr int NW = (WA_SINK_NW<T, DP>);
         constexpr size_t ws = (size_t)NW * (2 * img + 256), sum = 2ull * NW * DP * 32 * sizeof(float), lsk = ws > sum ? ws : sum;
-        const size_t blocks = (size_t)g.B * g.G * g.nst * g.nchunk;
-        GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
         GFS3D_ENSURE_LDS((wa_bwd_sink_kernel<T, DP>), lsk, who);
-        hipLaunchKernelGGL((wa_bwd_sink_kernel<T, DP>), dim3((unsigned)blocks), dim3(64 * NW), lsk, st, g);
+        hipLaunchKernelGGL((wa_bwd_sink_kernel<T, DP>), dim3((unsigned)sinks), dim3(64 * NW), lsk, st, g);
         GFS3D_LAUNCH_CHECK("wa_bwd_sink_kernel");
         if (g.nchunk > 1) {                                  // (then there are fewer than 1024 tiles)
             hipLaunchKernelGGL((wa_sink_sum_kernel<DP>), dim3(2 * DP * 32 / 1024, (unsigned)(g.B * g.G * g.nst)), dim3(256), 0, st, g.part, g.nchunk);
@@ -1082,7 +1086,8 @@ template <class T, int DP, bool WIDE> int wa_step_go(const WaArgs &g, void *out,
     constexpr size_t im = (size_t)NW * Mx<WaT<T>::PF>::NP * 32 * WaImg<DP>::ROWB, js = (size_t)NW * (64 + DP * 32) * sizeof(float), lds = im > js ? im : js;
     static_assert(lds <= 160 * 1024, "LDS");
     const size_t groups = (size_t)g.B * g.G * g.nblk, blocks = groups * g.nchunk;
-    GFS3D_REQUIRE(blocks < (1ull << 31), "%s: %zu workgroups", who, blocks);
+    WA_REQUIRE_GRID(blocks, 64 * NW, who);
+    if (g.nchunk > 1) WA_REQUIRE_GRID(groups, 8 * DP, who);
     GFS3D_ENSURE_LDS((wa_step_kernel<T, DP, WIDE>), lds, who);
     hipLaunchKernelGGL((wa_step_kernel<T, DP, WIDE>), dim3((unsigned)blocks), dim3(64 * NW), lds, st, g, (T *)out);
     GFS3D_LAUNCH_CHECK("wa_step_kernel");

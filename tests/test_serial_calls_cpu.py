@@ -82,3 +82,42 @@ def test_the_backward_s_workspace_is_bounded_by_its_tensors(B, N, H, G, D, left,
         floats += 8 * 2 * B * N * G * D
     need = _lib().gfs3d_window_attn_workspace_bytes(B, N, N, H, G, D, left, sinks, 0)
     assert 4 * B * H * N < need <= 4 * floats, (need, 4 * floats)
+
+
+def _attention_args(L, **kw):
+    import ctypes
+    from gfs3d import _lib as m
+    a = m.WindowAttnArgs()
+    a.B, a.N, a.S, a.H, a.G, a.D, a.type, a.scale = 1, 64, 64, 1, 1, 8, m.COMPUTE_BF16, 0.125
+    for name in ("q", "k", "v", "out", "lse", "dout", "dq", "dk", "dv", "workspace", "lengths"):
+        setattr(a, name, 4096)
+    for name in ("q_stride", "k_stride", "v_stride", "dout_stride"):
+        setattr(a, name, (ctypes.c_longlong * 3)(8, 8, 8))
+    a.workspace_bytes = 2 ** 62
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return ctypes.byref(a)
+
+
+@pytest.mark.parametrize("entry,kw", [
+    ("forward", dict(N=2 ** 29, S=2 ** 29, H=4)),                                # 2^24 workgroups of 256 threads
+    ("backward", dict(N=2 ** 29, S=2 ** 29, H=4)),
+    ("backward", dict(B=2 ** 19, N=1024, S=1024, sinks=1024)),                   # dQ and dK / dV fit, the sinks' tiles do not
+    ("backward", dict(B=2 ** 24, N=64, S=64, H=1)),
+    ("step", dict(B=2 ** 23, N=1, S=64)),
+])
+def test_calls_of_more_threads_than_a_launch_holds_are_refused_at_once(entry, kw):
+    """2^32 threads are refused by their number, before anything is launched (a launch here fails for want of a device)."""
+    L = _lib()
+    rc = getattr(L, f"gfs3d_window_attn_{entry}")(_attention_args(L, **kw), None)
+    assert rc == 1 and b"workgroups" in L.gfs3d_last_error(), (rc, L.gfs3d_last_error())
+
+
+def test_rotary_refuses_more_threads_than_a_launch_holds():
+    import ctypes
+    from gfs3d import _lib as m
+    L = _lib()
+    a = m.RotaryArgs()
+    a.B, a.N, a.D, a.type, a.q_heads, a.axes, a.pairs, a.magnitude = 2 ** 14, 2 ** 14, 2, 0, 1, 1, 1, 1.0
+    a.q = a.q_out = a.positions = a.freqs = 4096
+    assert L.gfs3d_rotary(ctypes.byref(a), None) == 1 and b"too many" in L.gfs3d_last_error(), L.gfs3d_last_error()
