@@ -1545,13 +1545,13 @@ def _window_inputs(a, q, k, v):
 
 class WindowAttentionFunction(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, left, right, sinks, scale, lengths):
+    def forward(ctx, q, k, v, left, right, sinks, scale, lengths, keep):
         a, lengths, device = _window_args("window_attention", q, k, v, left, right, sinks, scale, lengths)
         if a.S != a.N:
             raise RuntimeError(f"gfs3d.window_attention: q has {a.N} rows, k and v {a.S} (the last rows of a cache: window_attention_step)")
         q, k, v = _heads4(q), _heads4(k), _heads4(v)
         out = torch.empty((a.B, a.N, a.H, a.D), dtype=q.dtype, device=q.device)
-        grad = any(ctx.needs_input_grad[:3])
+        grad = keep and any(ctx.needs_input_grad[:3])            # (needs_input_grad says nothing of no_grad)
         lse = torch.empty((a.B, a.H, a.N), dtype=torch.float32, device=q.device) if grad else None
         low = torch.empty_like(out) if grad and out.element_size() == 2 else None
         if out.numel():
@@ -1581,7 +1581,7 @@ class WindowAttentionFunction(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)       # from torch's allocator: a captured graph keeps its own
             a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
             _launch("gfs3d_window_attn_backward", device, a)
-        return dq, dk, dv, None, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None, None
 
 
 def window_attention(q, k, v, left: Optional[int] = None, right: Optional[int] = None, sinks: int = 0,
@@ -1592,7 +1592,7 @@ def window_attention(q, k, v, left: Optional[int] = None, right: Optional[int] =
     is not read, its outputs and gradients are zero.  Keys and values in front of it have to be finite: a row next to a window takes
     part in products with zero weights.  scale defaults to D ** -0.5.  fp32, bf16 or half; D a multiple of 8 up to 128.
     Differentiable once (create_graph is refused), deterministic."""
-    return WindowAttentionFunction.apply(q, k, v, left, right, int(sinks), scale, lengths)
+    return WindowAttentionFunction.apply(q, k, v, left, right, int(sinks), scale, lengths, torch.is_grad_enabled())
 
 
 def window_attention_step(q, k, v, lengths, left: Optional[int] = None, sinks: int = 0, scale: Optional[float] = None) -> torch.Tensor:

@@ -121,3 +121,18 @@ def test_rotary_refuses_more_threads_than_a_launch_holds():
     a.B, a.N, a.D, a.type, a.q_heads, a.axes, a.pairs, a.magnitude = 2 ** 14, 2 ** 14, 2, 0, 1, 1, 1, 1.0
     a.q = a.q_out = a.positions = a.freqs = 4096
     assert L.gfs3d_rotary(ctypes.byref(a), None) == 1 and b"too many" in L.gfs3d_last_error(), L.gfs3d_last_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_window_attention_keeps_for_a_backward_only_where_one_can_follow(ops, dtype):
+    """Statistics and rounding remainders are written where a gradient is recorded, not for leaves under no_grad (an evaluation pass)."""
+    q, k, v = (torch.randn(1, 6, 2, 64, dtype=dtype) for _ in range(3))
+    kept = lambda: (ops.calls[-1][1].lse is not None, ops.calls[-1][1].out_low is not None)  # noqa: E731
+    ops.window_attention(q, k, v)
+    assert kept() == (False, False)
+    q.requires_grad_()
+    assert ops.window_attention(q, k, v).requires_grad and kept() == (True, dtype == torch.bfloat16)
+    for off in (torch.no_grad, torch.inference_mode):
+        with off():
+            out = ops.window_attention(q, k, v)
+        assert not out.requires_grad and kept() == (False, False)
