@@ -66,7 +66,6 @@ class WindowSelfAttention(nn.Module):
 
     def __init__(self, in_channel, out_channel=None, window=128, sinks=4, layers=1, heads=4, key_heads=2, head_dim=64):
         super().__init__()
-        from gfs3d import ops
         self.in_channel = in_channel
         self.out_channel = in_channel if out_channel is None else out_channel
         self.window, self.sinks, self.heads, self.key_heads, self.head_dim = int(window), int(sinks), heads, key_heads, head_dim
@@ -75,7 +74,17 @@ class WindowSelfAttention(nn.Module):
         self.qkv_maps = nn.ModuleList([nn.Linear(in_channel, wide, bias=False) for _ in range(layers)])
         self.out_maps = nn.ModuleList([nn.Linear(heads * head_dim, in_channel, bias=False) for _ in range(layers)])
         self.head_map = nn.Linear(in_channel, self.out_channel, bias=False)
-        self.register_buffer("freqs", ops.rotary_frequencies(head_dim // 2)[0], persistent=False)
+        self.register_buffer("freqs", self._frequencies(), persistent=False)
+
+    def _apply(self, fn, *args, **kwargs):
+        """Casts reach buffers too and round the frequencies (fp32: 7e-4 rad at position 65536): they are formed anew in 64 bits."""
+        super()._apply(fn, *args, **kwargs)
+        self.freqs = self._frequencies().to(self.freqs.device)
+        return self
+
+    def _frequencies(self):
+        from gfs3d import ops
+        return ops.rotary_frequencies(self.head_dim // 2)[0]
 
     def forward(self, x, cloud):
         """x (B, in_channel, N), cloud (B, C >= 3, N) -> (B, out_channel, N)."""
@@ -87,7 +96,6 @@ class WindowSelfAttention(nn.Module):
         from gfs3d.morton import morton_order
         order, rank = morton_order(cloud[:, :3].detach())
         place = torch.arange(x_pm.shape[1], device=x_pm.device, dtype=torch.int32)
-        freqs = self.freqs if self.freqs.dtype == torch.float64 else self.freqs.double()      # (module.float() reaches buffers too)
         dtype = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[ops.get_compute()]
         H, G, D = self.heads, self.key_heads, self.head_dim
         stream = x_pm.gather(1, order[:, :, None].expand(-1, -1, x_pm.shape[2]))
@@ -98,7 +106,7 @@ class WindowSelfAttention(nn.Module):
             else:
                 y, stream = ops.rms_norm(branch, norm, residual=stream)
             qkv = F.linear(y, qkv_map.weight.to(dtype)).unflatten(2, (H + 2 * G, D))
-            q, k = ops.rotary(qkv[:, :, :H], qkv[:, :, H:H + G], place, freqs)
+            q, k = ops.rotary(qkv[:, :, :H], qkv[:, :, H:H + G], place, self.freqs)
             o = ops.window_attention(q, k, qkv[:, :, H + G:], left=self.window, right=self.window, sinks=self.sinks)
             branch = F.linear(o.flatten(2), out_map.weight.to(dtype))
         y, _ = ops.rms_norm(branch, self.norms[len(self.qkv_maps)], residual=stream)

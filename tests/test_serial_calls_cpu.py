@@ -136,3 +136,17 @@ def test_window_attention_keeps_for_a_backward_only_where_one_can_follow(ops, dt
         with off():
             out = ops.window_attention(q, k, v)
         assert not out.requires_grad and kept() == (False, False)
+
+
+def test_the_learner_s_frequencies_stay_in_64_bits():
+    """Casts of the module (and of a model that holds it) round its weights, not the angles of its rotary positions."""
+    import copy
+    from gfs3d import ops as o
+    from model.attention import WindowSelfAttention
+    want = o.rotary_frequencies(32)[0]
+    m = WindowSelfAttention(64, 32, window=8)
+    for cast in (lambda x: x.float(), lambda x: x.half(), lambda x: x.to(torch.bfloat16), lambda x: x.double(), lambda x: x.to("cpu"),
+                 lambda x: torch.nn.Sequential(x).float()[0], copy.deepcopy):
+        m = cast(m)
+        assert m.freqs.dtype == torch.float64 and torch.equal(m.freqs, want)
+        assert "freqs" not in m.state_dict()
