@@ -66,6 +66,8 @@ class WindowSelfAttention(nn.Module):
 
     def __init__(self, in_channel, out_channel=None, window=128, sinks=4, layers=1, heads=4, key_heads=2, head_dim=64):
         super().__init__()
+        if layers < 1:
+            raise ValueError(f"WindowSelfAttention: layers must be at least 1, got {layers} (args.att_layers)")
         self.in_channel = in_channel
         self.out_channel = in_channel if out_channel is None else out_channel
         self.window, self.sinks, self.heads, self.key_heads, self.head_dim = int(window), int(sinks), heads, key_heads, head_dim

@@ -150,3 +150,16 @@ def test_the_learner_s_frequencies_stay_in_64_bits():
         m = cast(m)
         assert m.freqs.dtype == torch.float64 and torch.equal(m.freqs, want)
         assert "freqs" not in m.state_dict()
+
+
+def test_the_learner_refuses_to_have_no_layer():
+    """args.att_layers = 0 is refused where the model is built, not in its first forward."""
+    import types
+    from model.attention import SelfAttention, WindowSelfAttention, attention_learner
+    for layers in (0, -1):
+        with pytest.raises(ValueError, match="layers"):
+            WindowSelfAttention(64, 32, layers=layers)
+        with pytest.raises(ValueError, match="layers"):
+            attention_learner(types.SimpleNamespace(att_window=16, att_layers=layers), 64, 32)
+    assert type(attention_learner(types.SimpleNamespace(att_layers=0), 64, 32)) is SelfAttention
+    assert len(attention_learner(types.SimpleNamespace(att_window=16, att_layers=2), 64, 32).qkv_maps) == 2
