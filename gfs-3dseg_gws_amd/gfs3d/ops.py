@@ -1641,8 +1641,8 @@ def rotary_frequencies(pairs: int, base: float = 10000.0, scaling: Optional[str]
         if original_length is None or not original_length > 0 or not fast > slow > 0:
             raise ValueError("gfs3d.rotary_frequencies: \"parts\" needs original_length > 0 and fast > slow > 0")
         lo, hi = (pairs * math.log(original_length / (turns * 2 * math.pi)) / math.log(base) for turns in (fast, slow))
-        lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), pairs - 1)
-        ramp = ((p - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        lo, hi = max(math.floor(lo), 0), math.ceil(hi)
+        ramp = ((p - lo) / max(min(hi, pairs - 1) - lo, 1e-3)).clamp(0, 1) if hi > 0 else torch.ones_like(p)     # hi <= 0: the first pair, too
         freqs = freqs / factor * ramp + freqs * (1 - ramp)
         magnitude = 0.1 * math.log(factor) + 1.0
     elif scaling not in (None, "base"):

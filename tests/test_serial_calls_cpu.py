@@ -163,3 +163,21 @@ def test_the_learner_refuses_to_have_no_layer():
             attention_learner(types.SimpleNamespace(att_window=16, att_layers=layers), 64, 32)
     assert type(attention_learner(types.SimpleNamespace(att_layers=0), 64, 32)) is SelfAttention
     assert len(attention_learner(types.SimpleNamespace(att_window=16, att_layers=2), 64, 32).qkv_maps) == 2
+
+
+@pytest.mark.parametrize("length,fast,slow", [(4.0, 32.0, 1.0), (6.0, 32.0, 1.0), (6.5, 32.0, 1.0), (50.0, 40.0, 10.0), (64.0, 32.0, 1.0), (4096.0, 32.0, 1.0),
+                                              (1e6, 32.0, 1.0), (1e9, 2.0, 1.0)])
+@pytest.mark.parametrize("pairs", [1, 2, 10, 32])
+def test_parts_slow_every_pair_that_turns_too_seldom(length, fast, slow, pairs):
+    """Pairs that turn at most `slow` times over the original length are slowed by the whole factor, those that turn at least `fast` times
+    not at all, also where all of them or none do (short lengths: a room in metres)."""
+    import math
+    from gfs3d import ops as o
+    factor = 4.0
+    got, magnitude = o.rotary_frequencies(pairs, scaling="parts", factor=factor, original_length=length, fast=fast, slow=slow)
+    plain = o.rotary_frequencies(pairs)[0]
+    ratio, turns = plain / got, length * plain / (2 * math.pi)
+    assert abs(magnitude - (0.1 * math.log(factor) + 1)) < 1e-15
+    assert torch.allclose(ratio[turns <= slow], torch.full((), factor, dtype=torch.float64), rtol=1e-12), (ratio, turns)
+    assert torch.allclose(ratio[turns >= fast], torch.ones((), dtype=torch.float64), rtol=1e-12), (ratio, turns)
+    assert bool((ratio >= 1 - 1e-12).all()) and bool((ratio <= factor * (1 + 1e-12)).all()) and bool((ratio[1:] >= ratio[:-1] - 1e-12).all())
