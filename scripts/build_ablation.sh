@@ -5,7 +5,7 @@ set -eo pipefail
 src=$1; name=$2; shift 2
 pkg=$(dirname "$0")/../gfs-3dseg_gws_amd
 mkdir -p "$pkg/lib/abl"
-flags="--offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -Wno-unused-value"
+flags="--offload-arch=gfx950 -O3 -std=c++17 -ffp-contract=off -fPIC -Wno-unused-value -Xclang -target-feature -Xclang -packed-fp32-ops"       # as gfs3d/_lib.py
 /opt/rocm/bin/hipcc $flags "$@" -c "$pkg/csrc/$src" -o "$pkg/lib/abl/$name.o"
 objs=""
 for f in api knn edgeconv proto pointwise attention head kmeanspp optim; do

@@ -1,5 +1,5 @@
 // Micro-benchmark: v_mfma_f32_32x32x2_f32 throughput for a DEPENDENT chain on one accumulator vs independent
-// accumulators, at 1 / 2 / 4 waves per SIMD.   hipcc --offload-arch=gfx950 -O3 mfma_chain.hip -o mfma_chain
+// accumulators, at 1 / 2 / 4 waves per SIMD.   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_chain.hip -o mfma_chain
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 typedef float f32x16 __attribute__((ext_vector_type(16)));

@@ -1,6 +1,6 @@
 // Micro-benchmark: do an MFMA wave and a VALU wave that share a SIMD overlap?
 // Block = 512 threads = 8 waves = 2 per SIMD: waves 0-3 run dependent f32 MFMAs, waves 4-7 run v_fma_f32.
-// Times: MFMA only, VALU only, both.   hipcc --offload-arch=gfx950 -O3 mfma_valu_overlap.hip -o mfma_valu_overlap
+// Times: MFMA only, VALU only, both.   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops mfma_valu_overlap.hip -o mfma_valu_overlap
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 typedef float f32x16 __attribute__((ext_vector_type(16)));

@@ -1,5 +1,5 @@
 // ds_read_b64_tr_b16 semantics check (gfx950): per 16-lane group, lane 4q+p supplies the address of row q, columns 4p..4p+3;
-// lane i of the group receives column i of the 4 rows (element q = row q).   hipcc --offload-arch=gfx950 -O3 tr_read_check.hip -o tr_read_check
+// lane i of the group receives column i of the 4 rows (element q = row q).   hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tr_read_check.hip -o tr_read_check
 #include <hip/hip_runtime.h>
 #include <cstdio>
 typedef short s16x4 __attribute__((ext_vector_type(4)));

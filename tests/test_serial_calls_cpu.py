@@ -181,3 +181,16 @@ def test_parts_slow_every_pair_that_turns_too_seldom(length, fast, slow, pairs):
     assert torch.allclose(ratio[turns <= slow], torch.full((), factor, dtype=torch.float64), rtol=1e-12), (ratio, turns)
     assert torch.allclose(ratio[turns >= fast], torch.ones((), dtype=torch.float64), rtol=1e-12), (ratio, turns)
     assert bool((ratio >= 1 - 1e-12).all()) and bool((ratio <= factor * (1 + 1e-12)).all()) and bool((ratio[1:] >= ratio[:-1] - 1e-12).all())
+
+
+def test_every_build_of_the_kernels_leaves_packed_fp32_out():
+    """The library's flags, and each line of scripts/ that compiles device code or says how, keep packed fp32 instructions out."""
+    import pathlib
+    from gfs3d import _lib as m
+    flag = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+    assert flag in " ".join(m.HIPCC_FLAGS)
+    root = pathlib.Path(__file__).resolve().parent.parent / "scripts"
+    lines = [(f.name, line) for f in sorted(root.rglob("*")) if f.is_file() and f.suffix in (".sh", ".py", ".md", ".hip")
+             for line in f.read_text().splitlines() if "--offload-arch" in line]
+    assert len(lines) >= 5
+    assert not [x for x in lines if flag not in x[1]]
