@@ -194,3 +194,12 @@ def test_every_build_of_the_kernels_leaves_packed_fp32_out():
              for line in f.read_text().splitlines() if "--offload-arch" in line]
     assert len(lines) >= 5
     assert not [x for x in lines if flag not in x[1]]
+
+
+def test_build_compiles_also_where_a_library_is_there(monkeypatch):
+    import __graft_entry__
+    import gfs3d
+    asked = []
+    monkeypatch.setattr(gfs3d, "build_library", lambda force=False, verbose=False: asked.append(force) or gfs3d.library_path())
+    __graft_entry__.build()
+    assert asked == [True]
