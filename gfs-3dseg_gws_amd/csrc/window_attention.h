@@ -755,10 +755,9 @@ template <int DP> __global__ void __launch_bounds__(256) wa_sink_sum_kernel(floa
 // visible key tiles of a sequence are dealt to the waves of its nchunk workgroups in turn; each wave keeps its own running
 // softmax, the waves of a workgroup join through LDS, the workgroups (nchunk > 1) through part[..][m | l | O] and a second kernel.
 // HBM-bound: a wave has a tile of K and V in flight (32 keys x 128 channels: 16 KB) beside the one it computes.  64 sequences x 4112 keys
-// x 4 key heads x 128 bf16: 122 us, 4.4 TB/s; with lane masks around the loads of every tile 148.  WIDE: eight waves of one workgroup
-// share short caches, which saves the second launch (1028 keys x 64: 12.2 us for 15.2); otherwise 4, so that workgroups at
-// different stages share a CU.
-template <class T, int DP, bool WIDE> constexpr int WA_STEP_NW = WIDE && !(sizeof(T) == 4 && DP == 128) ? 8 : 4;
+// x 4 key heads x 128 bf16: 122 us, 4.4 TB/s; with lane masks around the loads of every tile 26 us more.  WIDE: eight waves instead of
+// four, for few small caches that are not split (see wa_step_plan).
+template <class T, int DP, bool WIDE> constexpr int WA_STEP_NW = WIDE ? 8 : 4;
 template <class T, int DP, bool WIDE>
 __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4 && DP == 128 ? 1 : 2) wa_step_kernel(const WaArgs g, T *__restrict__ out)
 {
@@ -789,7 +788,7 @@ __global__ void __launch_bounds__(64 * (WA_STEP_NW<T, DP, WIDE>), sizeof(T) == 4
     auto load = [&](int tt) {
         const int r0 = row0(tt);
         const T *kr = kb_ + (long long)(r0 + j) * g.ks.r, *vr = vb + (long long)(r0 + j) * g.vs.r;
-        if (r0 >= first && r0 + 32 <= len && g.D == DP) {                  // (masked loads of every tile: 148 us for 122, see above)
+        if (r0 >= first && r0 + 32 <= len && g.D == DP) {                  // (not masked: see above)
 #pragma unroll
             for (int kb = 0; kb < NK; ++kb) {
                 rk[kb] = wa_load8<T>(kr + 16 * kb + 8 * h);
@@ -992,16 +991,21 @@ void wa_dkv_plan(WaArgs &g, bool most = false)       // most: the bound over all
 }
 size_t wa_split_floats(const WaArgs &g) { return g.nsplit > 1 ? (size_t)g.nsplit * 2 * g.B * g.N * g.G * g.D : 0; }
 size_t wa_sink_floats(const WaArgs &g) { return (size_t)g.B * g.G * g.nst * g.nchunk * 2 * wa_dp(g.D) * 32; }
-// Short caches (at most 64 tiles): one workgroup of eight waves each and no second launch; else the keys are split until there are four
-// workgroups to a CU (64 x 4112 keys x 4 heads x 128: 122 us; two 155 with masked loads for 148, eight 128), four tiles to a wave at least
-void wa_step_plan(WaArgs &g, bool &wide)
+// Four waves to a workgroup, the keys split until every CU has one, two tiles to a wave at least (kernels alone, bf16, 4096 keys: 256
+// workgroups of 64 channels unsplit 51 us, in two 59, in four 65; of 128 channels 122, 122, 123; 512 of 128 channels unsplit 207, in two 223;
+// 16 x 2 key heads x 1024 x 128: 15.0, with twice the tiles per wave 18.5).  A split costs a second launch, 4 us of the caller's time: few
+// caches (fewer workgroups than CUs) of up to 320 KB take one workgroup of eight waves instead (whole calls, 4 x 2 key heads, 1028 keys x 64
+// bf16: 13.3 us for 17.7; the sides meet near 400 KB: 1024 x 128 bf16 20.7 for 17.6, 1024 x 64 fp32 22.0 for 17.7, 1536 x 32 fp32 17.7 for
+// 18.0; and with 256 x 2 key heads eight waves take 33.0 for 29.7).  Eight waves of fp32 at 128 channels do not fit a CU's LDS.
+constexpr long long WA_WIDE_BYTES = 320 * 1024;
+void wa_step_plan(WaArgs &g, bool fp32, bool &wide)
 {
     g.nblk = (int)(((long long)g.HG * g.N + 31) / 32);
     const long long keys = (long long)g.left + g.N < g.S ? (long long)g.left + g.N : g.S;
-    const long long tiles = keys / 32 + 2 + (g.sinks + 31) / 32, blocks = (long long)g.B * g.G * g.nblk;
-    wide = tiles <= 64;
-    long long n = wide ? 1 : (1024 + blocks - 1) / blocks;
-    if (n > tiles / 16) n = tiles / 16;
+    const long long tiles = keys / 32 + 2 + (g.sinks + 31) / 32, blocks = (long long)g.B * g.G * g.nblk, dp = wa_dp(g.D);
+    wide = blocks < 256 && tiles * 32 * dp * 2 * (fp32 ? 4 : 2) <= WA_WIDE_BYTES && !(fp32 && dp == 128);
+    long long n = wide ? 1 : (255 + blocks) / blocks;
+    if (n > tiles / 8) n = tiles / 8;
     g.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 // Waves of a workgroup in the forward: eight share every staged key tile where that leaves four workgroups to a CU (rooms of 2 x 65536 x
@@ -1099,7 +1103,10 @@ template <class T, int DP, bool WIDE> int wa_step_go(const WaArgs &g, void *out,
 }
 template <class T, int DP> int wa_step(const WaArgs &g, bool wide, void *out, hipStream_t st, const char *who)
 {
-    return wide ? wa_step_go<T, DP, true>(g, out, st, who) : wa_step_go<T, DP, false>(g, out, st, who);
+    if constexpr (!(sizeof(T) == 4 && DP == 128)) {
+        if (wide) return wa_step_go<T, DP, true>(g, out, st, who);
+    }
+    return wa_step_go<T, DP, false>(g, out, st, who);
 }
 
 // one call per (type, padded head size)
@@ -1127,7 +1134,7 @@ extern "C" size_t gfs3d_window_attn_workspace_bytes(int B, int N, int S, int H, 
     g.left = left < S ? left : S; g.sinks = sinks < S ? sinks : S;
     if (step) {
         bool wide;
-        wa_step_plan(g, wide);
+        wa_step_plan(g, step == 1 + GFS3D_COMPUTE_F32, wide);
         return g.nchunk > 1 ? (size_t)B * G * g.nblk * g.nchunk * (64 + wa_dp(D) * 32) * sizeof(float) : 0;
     }
     wa_sink_plan(g);
@@ -1173,8 +1180,8 @@ extern "C" int gfs3d_window_attn_step(const gfs3d_window_attn_args *a, void *str
     GFS3D_REQUIRE(a->lengths, "%s: NULL lengths", who);
     WaArgs g = wa_args(a);
     bool wide;
-    wa_step_plan(g, wide);
-    const size_t need = gfs3d_window_attn_workspace_bytes(a->B, a->N, a->S, a->H, a->G, a->D, a->left, a->sinks, 1);
+    wa_step_plan(g, a->type == GFS3D_COMPUTE_F32, wide);
+    const size_t need = gfs3d_window_attn_workspace_bytes(a->B, a->N, a->S, a->H, a->G, a->D, a->left, a->sinks, 1 + a->type);
     if (need > 0 && (!a->workspace || a->workspace_bytes < need)) {
         set_error("%s: workspace too small (%zu, needs %zu)", who, a->workspace_bytes, need);
         return GFS3D_ERR_WORKSPACE;

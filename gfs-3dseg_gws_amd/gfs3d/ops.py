@@ -1484,7 +1484,7 @@ def _no_grad_form(who: str, *tensors) -> None:
 
 def _first_order(who: str, *grads) -> None:
     """In a backward: gradients of gradients (create_graph=True, or forward mode through the backward) are refused, not left out."""
-    _no_tangents(f"{who}'s backward", *grads)
+    _no_tangents(who, *grads)
     if torch.is_grad_enabled():
         raise RuntimeError(f"gfs3d.{who}: the backward is not differentiable (create_graph=True)")
 
@@ -1610,7 +1610,7 @@ def window_attention_step(q, k, v, lengths, left: Optional[int] = None, sinks: i
     q, k, v = _heads4(q), _heads4(k), _heads4(v)
     _window_inputs(a, q, k, v)
     a.out = out.data_ptr()
-    nbytes = _lib.lib().gfs3d_window_attn_workspace_bytes(a.B, a.N, a.S, a.H, a.G, a.D, a.left, a.sinks, 1)
+    nbytes = _lib.lib().gfs3d_window_attn_workspace_bytes(a.B, a.N, a.S, a.H, a.G, a.D, a.left, a.sinks, 1 + a.type)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     if nbytes:
         a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes

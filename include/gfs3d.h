@@ -366,7 +366,8 @@ int gfs3d_attention_backward_mixed(const float *q, const float *k, const float *
  *   of q and k under a window of two keys are 3.7e-3 off for bf16, with it 2.5e-3; one rounding alone is 1.7e-3).
  * backward: dout -> dq, dk, dv; reads q, k, v, out, lse; deterministic (no atomics).
  * step: the N rows are the last positions of each sequence, row t at length - N + t; right is taken as 0 (S keys of capacity).
- * Workspace (device, 16-byte aligned): gfs3d_window_attn_workspace_bytes(..., step); 0 for the forward. */
+ * Workspace (device, 16-byte aligned): gfs3d_window_attn_workspace_bytes(..., step) with step 0 for the backward, 1 + type for the step (the
+ *   other types never need more than fp32's 1); none for the forward. */
 typedef struct gfs3d_window_attn_args {
     int B, N, S, H, G, D, type;
     int left, right, sinks;

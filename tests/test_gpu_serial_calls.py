@@ -79,3 +79,22 @@ def test_rotary_in_place(D, pairs, dtype, layout):
     for a, b in ((p, q), (r, k)):
         a, b = a.cpu().double(), b.cpu().double()
         assert float((a - b).abs().max()) <= 2 * (O.u(dtype) + 12 * O.U32) * 2 ** 0.5 * 2 ** 0.5 * float(b.abs().max())
+
+
+# B, T, S, H, G, D, left, sinks: either side of what one workgroup takes, for each type (320 KB of keys and values, 256 workgroups)
+SHORT = [
+    (2, 1, 1300, 8, 2, 64, 1100, 4), (2, 1, 1300, 8, 2, 64, 1200, 4), (2, 1, 1300, 8, 2, 64, 1290, 0), (1, 2, 640, 8, 2, 64, 560, 4),
+    (1, 1, 640, 4, 1, 128, 500, 4), (1, 1, 640, 4, 1, 128, 600, 4), (3, 3, 1100, 4, 1, 128, 1023, 33), (1, 1, 90, 4, 1, 128, None, 0),
+    (127, 1, 80, 2, 2, 32, 50, 1), (128, 1, 80, 2, 2, 32, 50, 1), (130, 1, 600, 2, 2, 32, 500, 1), (100, 1, 700, 2, 2, 64, None, 3),
+    (40, 1, 1500, 2, 2, 16, 1400, 3),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", range(len(SHORT)))
+def test_step_at_the_borders_of_its_plan(case, dtype):
+    B, T, S, H, G, D, left, sinks = SHORT[case]
+    q, k, v = rnd(40, (B, T, H, D), dtype), rnd(41, (B, S, G, D), dtype), rnd(42, (B, S, G, D), dtype)
+    lens = [max(0, S - 37 * (b % 40)) for b in range(B)]
+    out = ops().window_attention_step(q, k, v, torch.tensor(lens, dtype=torch.int32, device="cuda"), left=left, sinks=sinks)
+    O.check(f"{dtype} {SHORT[case]}", out, O.attention(q, k, v, left, 0, sinks, lens, step=True, dtype=dtype)["out"])
