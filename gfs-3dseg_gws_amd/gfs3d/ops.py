@@ -1697,7 +1697,7 @@ def rotary(q, k, positions, freqs, magnitude: float = 1.0, layout: str = "half")
     channels, turns by the angle positions[.., a] freqs[p] and is multiplied by `magnitude`; channels behind the sections are
     copied.  layout "half": pair p is the section's channels (p, P + p); "interleaved": (2 p, 2 p + 1).  positions (N,), (B, N) or
     (B, N, axes) with 1 to 3 axes (a point's coordinates, say), int32, int64 or float32; freqs (P,) float64 on the device
-    (`rotary_frequencies`); angles are formed in float64.  Differentiable in q and k.  Returns (q', k'), or q' alone without k."""
+    (`rotary_frequencies`); angles are formed in float64.  Differentiable in q and k (positions or freqs that require a gradient are refused).  Returns (q', k'), or q' alone without k."""
     device = _need_typed("rotary", q) if k is None else _need_typed("rotary", q, k)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise RuntimeError("gfs3d.rotary: q must be (B, N, H, D) and k (B, N, G, D)")
@@ -1718,6 +1718,8 @@ def rotary(q, k, positions, freqs, magnitude: float = 1.0, layout: str = "half")
     if P < 1 or 2 * P > D or P > 1024 or H < 1 or (k is not None and k.shape[2] < 1):
         raise RuntimeError(f"gfs3d.rotary: {axes} axes of {freqs.shape[0]} pairs do not fit heads of {D} channels")
     _no_tangents("rotary", q, k, positions, freqs)
+    if (positions.requires_grad or freqs.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError("gfs3d.rotary has no gradient for positions and freqs: detach them")
     positions, freqs = positions.contiguous(), freqs.contiguous()
     interleaved = 1 if layout == "interleaved" else 0
     if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():

@@ -216,3 +216,16 @@ def test_short_caches_are_split_where_one_workgroup_is_too_few():
     assert need(256, 1, 2048, 8, 2, 64, 1023, 4, bf16) == 0 and need(64, 1, 8192, 32, 4, 128, 4095, 16, bf16) == 0
     for case in ((4, 1, 2048, 8, 2, 64, 1023, 4), (3, 2, 9000, 16, 2, 128, 8191, 40), (1, 5, 600, 8, 1, 32, 500, 7)):
         assert need(*case, f32) >= need(*case, bf16) == need(*case, 3)
+
+
+@pytest.mark.parametrize("name", ["positions", "freqs"])
+def test_rotary_refuses_to_leave_out_the_gradient_of_positions(ops, name):
+    """Coordinates that are learnt, or frequencies, would silently miss their share of the gradient: the call says so; detached they pass."""
+    t = _inputs(ops)
+    t["q"].requires_grad_(), t[name].requires_grad_()
+    with pytest.raises(RuntimeError, match="detach"):
+        CALLS["rotary"][1](ops, t)
+    with torch.no_grad():
+        CALLS["rotary"][1](ops, t)
+    t[name] = t[name].detach()
+    assert CALLS["rotary"][1](ops, t)[0].requires_grad
