@@ -109,8 +109,9 @@ __device__ __forceinline__ unsigned pack_hi16(unsigned a, unsigned b) { return _
 //   PREC_BF16 ONE bf16 product per fp32 product: operands rounded to nearest-even bf16 (8 significand bits), fp32 accumulate
 //   PREC_F16  the same with IEEE half operands (11 significand bits; forward passes only - gradients underflow in half)
 // All three use the same LDS row images ([piece 0 | piece 1 | piece 2 | pad]); the reduced forms fill and read piece 0 only.
-//   PREC_X3   (internal: screens with an error bound, never a result) operands as hi + mid round-to-nearest bf16 pairs, the three
-//             products hi hi + hi mid + mid hi: ~2^-15 |x||y| per product dropped (the screened kNN's form, knn.hip)
+//   PREC_X3   (internal) operands as hi + mid round-to-nearest bf16 pairs, the three products hi hi + hi mid + mid hi: ~2^-15 |x||y| per
+//             product dropped.  Screens with an error bound (the screened kNN, knn.hip; the k-means assignment, proto.hip) and the
+//             gradients of half tensors in window attention, whose values two pieces hold exactly and whose range half does not hold
 enum { PREC_X6 = GFS3D_COMPUTE_F32, PREC_BF16 = GFS3D_COMPUTE_BF16, PREC_F16 = GFS3D_COMPUTE_F16, PREC_X3 = 3 };
 typedef float mm_f32x16 __attribute__((ext_vector_type(16)));
 typedef float mm_f32x2 __attribute__((ext_vector_type(2)));

@@ -5,12 +5,13 @@
 // The angle is formed and reduced to an eighth of a turn in fp64 (a position of 10^6 in fp32 is off by 0.06 rad), its sine and cosine are
 // Taylor sums in fp32 there (next term below 2e-9); both are computed once per (token, pair) into LDS and serve all heads of q and k,
 // which the same launch rotates.  The backward is the same kernel with the sine's sign turned.  HBM-bound: each value is read and
-// written once, in 16-byte accesses (2 x 65536 tokens x 16 heads x 64 bf16: 105 us, 5.1 TB/s; 32 x 2048 x 8 x 64 fp32: 58 us, 4.6).
+// written once, in 16-byte accesses (2 x 65536 tokens x 16 heads x 64 bf16: 107 us, 5.0 TB/s; 32 x 2048 x 8 x 64 fp32: 63 us, 4.3).
 //
 // K9 root-mean-square norm with the residual's addition:  s = round(x + r),  y = s (mean s^2 + eps)^-1/2 w
 // A group of 8 .. 256 lanes holds a row in registers (8 consecutive channels per lane and step), so that it is read once; the sum
 // of squares, the maximum of |y| for the 8-bit form, and the backward's mean of dy w s are reductions over the group.  HBM-bound:
-// 65536 x 256 bf16 beside an fp32 stream 37 us forward (5.4 TB/s), 46 us backward (5.8); 16384 x 4096 half to e4m3 100 us (4.7).
+// 65536 x 256 bf16 beside an fp32 stream 38 us forward (5.3 TB/s), 46 us backward (5.8); 16384 x 4096 half to e4m3 102 - 104 us (4.6).  Rows that
+// are no multiple of 8 channels, or not aligned, are read element by element: 4097 x 4095 123 and 148 us, 4096 x 4096 40 and 51.
 
 namespace gfs3d {
 namespace {

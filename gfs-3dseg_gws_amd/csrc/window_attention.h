@@ -17,9 +17,12 @@
 // Scores, softmax statistics, accumulators and all sums over heads or chunks are fp32.  Probabilities and dS are rounded to the operand
 // type of the matrix cores: bf16 / half for those tensors, exact 3-way bf16 splits (PREC_X6) for fp32; the gradients of half
 // tensors take two bf16 pieces (PREC_X3), whose range is fp32's - a mean loss underflows in half.
-// Measured (2 x 65536 rows, 8 heads x 64, bf16, 512 to either side + 16 sinks): forward 420 us (0.67 PFLOP/s of visible pairs), dQ 580
-// (0.72), dK / dV 780 (0.72), sinks 75.  Bound by vector issue: of a forward tile's cycles the vector pipe is busy 64 %, the matrix
-// pipe 32 %, and four waves per SIMD (128 registers) did better than every form that overlaps the two within a wave at two.
+// Measured (2 x 65536 rows, 8 heads x 64, 512 to either side + 16 sinks; medians of a warm device, three cards): bf16 forward 400 - 427 us
+// (0.65 - 0.70 PFLOP/s of visible pairs), dQ 540 - 575 (0.73 - 0.77), dK / dV 730 - 776 (0.72 - 0.76), sinks 71; half 402, 1100, 1520, 136 (three
+// products for one in the backward) on the fastest of them; fp32, a quarter of the rows: 395, 516, 663, 58.  In the bf16 forward the vector pipe is busy 64 % of the time, the matrix pipe 32 %, and
+// 30 % of the LDS's active cycles are bank conflicts; four waves per SIMD (128 registers) did better than every form that overlaps the
+// pipes within a wave at two.  Head sizes other than 32, 64 and 128 are padded to the next of them in every product, and their loads
+// are masked by channel (7 x 1777 rows x 6 / 2 heads, forward: 40 channels 61.5 us, 64 channels 61; 80 and 96 channels 127, as 128).
 
 namespace gfs3d {
 namespace {
@@ -43,8 +46,8 @@ template <class T> struct WaT;
 template <> struct WaT<float> { static constexpr int PF = PREC_X6, PB = PREC_X6; };
 template <> struct WaT<__bf16> { static constexpr int PF = PREC_BF16, PB = PREC_BF16; };
 template <> struct WaT<_Float16> { static constexpr int PF = PREC_F16, PB = PREC_X3; };
-// keys of a staged tile in the forward (eight waves, 128 channels: causal 8192 x 16 heads half 655 us with 128 keys, 672 with 64; 64
-// channels: no difference)
+// keys of a staged tile in the forward (eight waves, 128 channels: 4 x 8192 rows x 16 / 4 heads half, causal over 2048: 568 us with 128 keys, 593
+// with 64; 64 channels: no difference)
 template <class T, int DP, int NW> constexpr int WA_KT = sizeof(T) == 4 ? 32 : NW == 8 && DP == 128 ? 128 : 64;
 
 // eight consecutive channels as they lie in memory
@@ -980,7 +983,8 @@ void wa_sink_plan(WaArgs &g)
     if (keys > 0 && n > (1023 + keys) / keys) n = (1023 + keys) / keys;
     g.nchunk = (int)(n < 1 ? 1 : n);
 }
-// dK, dV: workgroups of 128 keys, their turns split until every CU has two workgroups (at most 8 ways, 4 turns at least)
+// dK, dV: workgroups of 128 keys, their turns split until every CU has two workgroups (at most 8 ways, 4 turns at least; 196 workgroups of 7 x
+// 1777 rows x 6 / 2 heads x 40, three ways: 116 us + 6 for the join, unsplit 157)
 void wa_dkv_plan(WaArgs &g, bool most = false)       // most: the bound over all types and reaches
 {
     const long long blocks = (long long)g.B * g.G * ((g.N + 127) / 128);
@@ -1009,7 +1013,8 @@ void wa_step_plan(WaArgs &g, bool fp32, bool &wide)
     g.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 // Waves of a workgroup in the forward: eight share every staged key tile where that leaves four workgroups to a CU (rooms of 2 x 65536 x
-// 8 heads x 64: 405 us, with four waves 422; dQ in eight waves spills at four waves per SIMD: 659 us for 561), four otherwise
+// 8 heads x 64: 409 us, with four waves 418; 128 channels, causal: 568, with four 600; dQ in eight waves spills at four waves per SIMD and
+// was 17 % slower), four otherwise
 template <class T, int DP> bool wa_wide(const WaArgs &g)
 {
     return sizeof(T) == 2 && (long long)g.B * g.G * (((g.N + 31) / 32 * (long long)g.HG + 7) / 8) >= 1024;

@@ -7,9 +7,12 @@ MEASURED NEUTRAL (round 5, DESIGN_HISTORY.md): delivering the c2 blocks in this 
 (their rows are L2-resident per XCD either way: ec_stats1 44.5 vs 43.4 us, ec_main_fwd 104.1 vs 103.5, ec_main_bwd_pair 217.6 vs
 213.6, csr_gather 91.4 vs 90.8). The first run of the experiment also broke the screened kNN (its buckets were runs of consecutive
 points, so the neighbours of a sorted cloud shared buckets and the lists overflowed: knn_exact_kernel 45 -> 775 us); csrc/knn.hip
-now strides and rotates its stages over the cloud and is indifferent to the order (42 vs 44 us). Kept as the reproduction knob of
-the experiment (`GFS3D_BENCH_MORTON=1 python bench.py`, scripts/exp_morton_locality.py); the product path keeps the sampled order
-the reference's loader produces (dataloaders/loader.py:64-82)."""
+now strides and rotates its stages over the cloud and is indifferent to the order (42 vs 44 us). Those kernels therefore keep the
+sampled order that the reference's loader produces (dataloaders/loader.py:64-82); the experiment's knob is `GFS3D_BENCH_MORTON=1 python
+bench.py`, scripts/exp_morton_locality.py.
+
+model.attention.WindowSelfAttention (args.att_window) puts its points in this order in every forward. It is some 120 small launches of
+the tensor library: 0.81 ms for 32 x 2048 points and 0.85 for 2 x 65536, most of the layer's forward (1.05 and 1.57 ms in fp32)."""
 from __future__ import annotations
 
 import torch

@@ -354,7 +354,8 @@ int gfs3d_attention_backward_mixed(const float *q, const float *k, const float *
  *     out_i = sum_j p_ij v_j,  p_i. = softmax over the visible j of  scale q_i . k_j
  *     j visible to i:  i, j < length  and  j <= i + right  and  (j >= i - left  or  j < sinks)
  * Rows that see nothing (those at or behind their sequence's length among them) are zero, and so are their gradients; what lies
- * behind a sequence's length is not read.
+ * behind a sequence's length is not read; in front of it keys, values, queries and dout have to be finite (a row next to a window takes
+ * part in products with zero weights).
  *   q (B, N, H, D), k / v (B, S, G, D): any strides (sequence, row, head; in elements, multiples of 16 bytes, >= 0, rows
  *   at most 2^23 apart) with dense channels, 16-byte aligned; head h reads key head h / (H / G).  D a multiple of 8 up to 128.  out, dq (B, N, H, D) and dk, dv
  *   (B, N, G, D) are dense.  type: element type of all of them, named as the GFS3D_COMPUTE_* ids (the arithmetic follows it: fp32 at
