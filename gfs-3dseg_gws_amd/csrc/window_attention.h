@@ -995,21 +995,26 @@ void wa_dkv_plan(WaArgs &g, bool most = false)       // most: the bound over all
 }
 size_t wa_split_floats(const WaArgs &g) { return g.nsplit > 1 ? (size_t)g.nsplit * 2 * g.B * g.N * g.G * g.D : 0; }
 size_t wa_sink_floats(const WaArgs &g) { return (size_t)g.B * g.G * g.nst * g.nchunk * 2 * wa_dp(g.D) * 32; }
-// Four waves to a workgroup, the keys split until every CU has one, two tiles to a wave at least (kernels alone, bf16, 4096 keys: 256
-// workgroups of 64 channels unsplit 51 us, in two 59, in four 65; of 128 channels 122, 122, 123; 512 of 128 channels unsplit 207, in two 223;
-// 16 x 2 key heads x 1024 x 128: 15.0, with twice the tiles per wave 18.5).  A split costs a second launch, 4 us of the caller's time: few
-// caches (fewer workgroups than CUs) of up to 320 KB take one workgroup of eight waves instead (whole calls, 4 x 2 key heads, 1028 keys x 64
-// bf16: 13.3 us for 17.7; the sides meet near 400 KB: 1024 x 128 bf16 20.7 for 17.6, 1024 x 64 fp32 22.0 for 17.7, 1536 x 32 fp32 17.7 for
-// 18.0; and with 256 x 2 key heads eight waves take 33.0 for 29.7).  Eight waves of fp32 at 128 channels do not fit a CU's LDS.
+// Long caches (more than 64 tiles): four waves to a workgroup, the keys split until every CU has four, four tiles to a wave at least.  Lengths
+// differ in earnest, and the longest sequence must not be one workgroup's (kernels, 64 sequences x 4 key heads x 128 bf16: lengths spread over
+// 400 .. 8192 153 us, unsplit 204; one of 8192 beside 409 48 for 128; all of 8192 223 for 244.  256 x 2 x 64, all of 8192: 237 for 209).
+// Short caches: split until every CU has one workgroup, two tiles to a wave at least (16 x 2 key heads x 1028 x 128 bf16: 15.0 us, with twice the
+// tiles per wave 18.5; 256 x 2 x 1028 x 64: unsplit 29.7, in two 38.9).  A split costs a second launch, 4 us of the caller's time: caches of
+// up to 320 KB take one workgroup of eight waves instead (whole calls, 4 x 2 key heads, 1028 keys x 64 bf16: 13.3 us for 17.7; the sides meet
+// near 400 KB: 1028 x 128 bf16 20.7 for 17.6, 1028 x 64 fp32 22.0 for 17.7, 1540 x 32 fp32 17.7 for 18.0).  With a workgroup for every CU
+// nothing is split, and eight waves serve a long sequence beside short ones better (256 x 2 key heads of up to 1900 x 64 bf16, every eighth full:
+// 24 us for 33; all full: 56 for 53) unless they have fewer than two tiles each and a CU has two workgroups (260 keys, 512 workgroups x 64 bf16:
+// 14.7 for 10.0; 256 x 64 fp32: 12.4 for 14.2).  Eight waves of fp32 at 128 channels do not fit a CU's LDS.
 constexpr long long WA_WIDE_BYTES = 320 * 1024;
 void wa_step_plan(WaArgs &g, bool fp32, bool &wide)
 {
     g.nblk = (int)(((long long)g.HG * g.N + 31) / 32);
     const long long keys = (long long)g.left + g.N < g.S ? (long long)g.left + g.N : g.S;
     const long long tiles = keys / 32 + 2 + (g.sinks + 31) / 32, blocks = (long long)g.B * g.G * g.nblk, dp = wa_dp(g.D);
-    wide = blocks < 256 && tiles * 32 * dp * 2 * (fp32 ? 4 : 2) <= WA_WIDE_BYTES && !(fp32 && dp == 128);
-    long long n = wide ? 1 : (255 + blocks) / blocks;
-    if (n > tiles / 8) n = tiles / 8;
+    const bool longs = tiles > 64;
+    wide = !longs && !(fp32 && dp == 128) && (blocks < 256 ? tiles * 32 * dp * 2 * (fp32 ? 4 : 2) <= WA_WIDE_BYTES : tiles > 16 || blocks < 512);
+    long long n = wide ? 1 : ((longs ? 1023 : 255) + blocks) / blocks;
+    if (n > tiles / (longs ? 16 : 8)) n = tiles / (longs ? 16 : 8);
     g.nchunk = (int)(n < 1 ? 1 : n > 64 ? 64 : n);
 }
 // Waves of a workgroup in the forward: eight share every staged key tile where that leaves four workgroups to a CU (rooms of 2 x 65536 x

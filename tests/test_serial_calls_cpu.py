@@ -207,13 +207,14 @@ def test_build_compiles_also_where_a_library_is_there(monkeypatch):
 
 def test_short_caches_are_split_where_one_workgroup_is_too_few():
     """The step's plan, seen through its workspace: one workgroup per key head only for few small caches; fp32 heads of 128 channels, wide
-    16-bit caches and long ones are split; as many sequences as CUs are not."""
+    16-bit caches and long ones are split; as many short ones as CUs are not."""
     need = _lib().gfs3d_window_attn_workspace_bytes
     f32, bf16 = 1, 2                                          # step: 1 + GFS3D_COMPUTE_*
     assert need(4, 1, 2048, 8, 2, 64, 1023, 4, bf16) == 0 and need(4, 1, 2048, 8, 2, 64, 255, 4, f32) == 0
     assert need(4, 1, 2048, 8, 2, 64, 1023, 4, f32) > 0       # 526 KB a key head
     assert need(1, 1, 2048, 8, 2, 128, 1023, 4, bf16) > 0 and need(4, 1, 2048, 8, 2, 128, 1023, 4, f32) > 0
-    assert need(256, 1, 2048, 8, 2, 64, 1023, 4, bf16) == 0 and need(64, 1, 8192, 32, 4, 128, 4095, 16, bf16) == 0
+    assert need(256, 1, 2048, 8, 2, 64, 1023, 4, bf16) == 0
+    assert need(64, 1, 8192, 32, 4, 128, 4095, 16, bf16) == need(64, 1, 8192, 32, 4, 128, 4095, 16, f32) > 0     # lengths differ: four to a CU
     for case in ((4, 1, 2048, 8, 2, 64, 1023, 4), (3, 2, 9000, 16, 2, 128, 8191, 40), (1, 5, 600, 8, 1, 32, 500, 7)):
         assert need(*case, f32) >= need(*case, bf16) == need(*case, 3)
 
