@@ -368,7 +368,8 @@ int gfs3d_attention_backward_mixed(const float *q, const float *k, const float *
  * backward: dout -> dq, dk, dv; reads q, k, v, out, lse; deterministic (no atomics).
  * step: the N rows are the last positions of each sequence, row t at length - N + t; right is taken as 0 (S keys of capacity).
  * Workspace (device, 16-byte aligned): gfs3d_window_attn_workspace_bytes(..., step) with step 0 for the backward, 1 + type for the step (the
- *   other types never need more than fp32's 1); none for the forward. */
+ *   other types never need more than fp32's 1); none for the forward.  Calls that would take 2^32 threads in one launch are refused
+ *   before anything runs (about 2^24 times 128 (row, head) pairs); so are K8's. */
 typedef struct gfs3d_window_attn_args {
     int B, N, S, H, G, D, type;
     int left, right, sinks;
